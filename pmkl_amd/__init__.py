@@ -8,6 +8,9 @@ Drop-in replacement for pmkl's attention path:
 and for the row softmax the fused kernel replaces:
   * C++:    include/pmkl/norm/warp_softmax.h     (pmkl::norm::warp_softmax_forward)
   * C ABI:  include/pmkl_softmax.h               (libpmkl_attn.so)
+and, for serving, attention over a key and value cache in 8 bits:
+  * C ABI:  include/pmkl_cache.h                 (libpmkl_attn.so)
+  * torch:  `cache_slots`, `cache_append` and `cache_attn_fwd` below
 
 `attn_fwd`, `attn_bwd`, `warp_softmax_forward` and `softmax` below call the C
 ABI directly on device tensors through ctypes; they are what the parity tests
@@ -17,7 +20,8 @@ from __future__ import annotations
 
 from . import capi
 
-__all__ = ["attn_fwd", "attn_bwd", "warp_softmax_forward", "softmax", "capi", "torch_dtype_to_pmkl"]
+__all__ = ["attn_fwd", "attn_bwd", "warp_softmax_forward", "softmax", "cache_slots", "cache_append",
+           "cache_attn_fwd", "capi", "torch_dtype_to_pmkl"]
 
 
 def torch_dtype_to_pmkl(dt) -> int:
@@ -246,3 +250,63 @@ def softmax(x, is_log: bool = False, out_dtype=None, stream=None):
     if rc != capi.PMKL_OK:
         raise capi.PmklError(rc, capi.last_error())
     return out.view(x.shape)
+
+
+def cache_slots(cached_lens, new_lens, block_table, free_pages, free_head, page_size: int, num_tokens: int):
+    """Block table entries and slots of a serving step's tokens, through pmkl_cache_slots.
+
+    Request b holds cached_lens[b] tokens (int32 [B]) and gets new_lens[b] more.
+    The pages that it needs for them are free_pages[free_head], free_pages[free_head
+    + 1], ... in the order of the requests (int32 [F] and [1]); they are entered
+    into its row of block_table (int32 [B, W], in place).  Returns
+      seq_lens     int32 [B]      cached + new
+      query_start  int32 [B + 1]  first token of each request, and their number
+      slots        int64 [num_tokens]  page * page_size + offset of every new token, in the requests' order;
+                   -1 for rows past the last token
+      free_head    int32 [1]      free_head plus the pages taken
+    num_tokens is the sum of new_lens, or more.  Where the list or a table row is
+    too short, the tokens concerned have slot -1 (pmkl_cache.h says more); the
+    returned free_head is then past F in the first case.  On torch's current stream;
+    nothing is synchronised.
+    """
+    from . import pmkl_pytorch_ext
+
+    return pmkl_pytorch_ext.cache_slots(cached_lens, new_lens, block_table, free_pages, free_head, page_size, num_tokens)
+
+
+def cache_append(k, v, slots, k_cache, v_cache, k_scale, v_scale) -> None:
+    """New keys and values into the cache, in place, through pmkl_cache_append.
+
+    k, v: [N, kv_heads, head_dim] (float32, float16 or bfloat16; views of a packed
+    projection are read as they are); slots: int64 [N], from cache_slots, tokens of
+    slots outside the cache are skipped.  k_cache: float8_e4m3fn [pages, kv_heads,
+    page_size, head_dim]; v_cache: [pages, kv_heads, head_dim, page_size]; k_scale,
+    v_scale: float32 [pages, kv_heads].  A page's scale is the least power of two
+    under which its values are at most 448; where a new token needs a larger one,
+    the page's earlier codes are made anew from their values.  Each page may get
+    tokens of one request in a call.  On torch's current stream.
+    """
+    from . import pmkl_pytorch_ext
+
+    pmkl_pytorch_ext.cache_append(k, v, slots, k_cache, v_cache, k_scale, v_scale)
+
+
+def cache_attn_fwd(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_start, is_causal: bool = True,
+                   scale: float | None = None, out=None, out_m=None, out_l=None):
+    """Attention of the requests' newest tokens over the cache, through pmkl_cache_attn_fwd.
+
+    q: [N, heads, head_dim] (float32, float16 or bfloat16), the requests' tokens one
+    after the other; request b has rows query_start[b] .. query_start[b + 1] - 1, the
+    last of its seq_lens[b] tokens in the cache.  heads is a multiple of kv_heads:
+    query head h reads key head h // (heads // kv_heads).  The cache as for
+    cache_append, block_table int32 [B, W].  is_causal: a token sees itself and what
+    lies before it, else all of its request.  scale: 1/sqrt(head_dim) by default.
+    Returns (out, out_m, out_l): out in q's dtype, the row max and row sum [N, heads] in
+    float32; given buffers are written and returned.  A row that sees no token has
+    out 0, out_m -inf and out_l 0; rows of no request are not written.  On torch's
+    current stream, with workspace from its allocator.  No backward.
+    """
+    from . import pmkl_pytorch_ext
+
+    return pmkl_pytorch_ext.cache_attn_fwd(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_start,
+                                           is_causal, scale, out, out_m, out_l)

@@ -1,5 +1,5 @@
-"""ctypes view of the C ABI in include/pmkl_attn.h and include/pmkl_softmax.h
-(libpmkl_attn.so).
+"""ctypes view of the C ABI in include/pmkl_attn.h, include/pmkl_softmax.h and
+include/pmkl_cache.h (libpmkl_attn.so).
 
 This is the thin Python handle on the drop-in boundary: it passes device
 pointers, sizes and a HIP stream, nothing else.  Loading fails loudly when the
@@ -39,6 +39,15 @@ EXPORTED_SYMBOLS = (
     "pmkl_abi_version",
     "pmkl_softmax_fwd",
     "pmkl_warp_softmax_forward",
+)
+
+# Every symbol include/pmkl_cache.h declares.
+CACHE_SYMBOLS = (
+    "pmkl_cache_slots",
+    "pmkl_cache_append",
+    "pmkl_cache_attn_fwd",
+    "pmkl_cache_attn_workspace_size",
+    "pmkl_cache_attn_kernel_name",
 )
 
 
@@ -120,6 +129,89 @@ class SoftmaxArgs(ctypes.Structure):
     ]
 
 
+class KvCache(ctypes.Structure):
+    """Mirror of pmkl_kv_cache."""
+
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("pages", ctypes.c_int64),
+        ("kv_heads", ctypes.c_int64),
+        ("page_size", ctypes.c_int64),
+        ("head_dim", ctypes.c_int64),
+        ("k_strides", ctypes.c_int64 * 3),
+        ("v_strides", ctypes.c_int64 * 3),
+        ("k_scale_strides", ctypes.c_int64 * 2),
+        ("v_scale_strides", ctypes.c_int64 * 2),
+    ]
+
+
+class CacheSlotsArgs(ctypes.Structure):
+    """Mirror of pmkl_cache_slots_args."""
+
+    _fields_ = [
+        ("cached_lens", ctypes.c_void_p),
+        ("new_lens", ctypes.c_void_p),
+        ("block_table", ctypes.c_void_p),
+        ("free_pages", ctypes.c_void_p),
+        ("free_head", ctypes.c_void_p),
+        ("seq_lens", ctypes.c_void_p),
+        ("query_start", ctypes.c_void_p),
+        ("slots", ctypes.c_void_p),
+        ("free_head_out", ctypes.c_void_p),
+        ("batch", ctypes.c_int64),
+        ("table_width", ctypes.c_int64),
+        ("table_stride", ctypes.c_int64),
+        ("free_count", ctypes.c_int64),
+        ("page_size", ctypes.c_int64),
+        ("tokens", ctypes.c_int64),
+    ]
+
+
+class CacheAppendArgs(ctypes.Structure):
+    """Mirror of pmkl_cache_append_args."""
+
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("slots", ctypes.c_void_p),
+        ("cache", KvCache),
+        ("dtype", ctypes.c_int32),
+        ("tokens", ctypes.c_int64),
+        ("k_strides", ctypes.c_int64 * 2),
+        ("v_strides", ctypes.c_int64 * 2),
+    ]
+
+
+class CacheAttnArgs(ctypes.Structure):
+    """Mirror of pmkl_cache_attn_args."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("o", ctypes.c_void_p),
+        ("m", ctypes.c_void_p),
+        ("l", ctypes.c_void_p),
+        ("cache", KvCache),
+        ("block_table", ctypes.c_void_p),
+        ("seq_lens", ctypes.c_void_p),
+        ("query_start", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_uint64),
+        ("dtype", ctypes.c_int32),
+        ("is_causal", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("tokens", ctypes.c_int64),
+        ("heads", ctypes.c_int64),
+        ("batch", ctypes.c_int64),
+        ("table_width", ctypes.c_int64),
+        ("table_stride", ctypes.c_int64),
+        ("q_strides", ctypes.c_int64 * 2),
+        ("o_strides", ctypes.c_int64 * 2),
+    ]
+
+
 class PmklError(RuntimeError):
     def __init__(self, code: int, msg: str):
         super().__init__(f"pmkl error {code}: {msg}")
@@ -170,6 +262,14 @@ def load() -> ctypes.CDLL:
         ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p,
     ]
     lib.pmkl_warp_softmax_forward.restype = ctypes.c_int
+    for name, cls in (("pmkl_cache_slots", CacheSlotsArgs), ("pmkl_cache_append", CacheAppendArgs),
+                      ("pmkl_cache_attn_fwd", CacheAttnArgs)):
+        getattr(lib, name).argtypes = [ctypes.POINTER(cls), ctypes.c_void_p]
+        getattr(lib, name).restype = ctypes.c_int
+    lib.pmkl_cache_attn_workspace_size.argtypes = [ctypes.POINTER(CacheAttnArgs)]
+    lib.pmkl_cache_attn_workspace_size.restype = ctypes.c_uint64
+    lib.pmkl_cache_attn_kernel_name.argtypes = [ctypes.POINTER(CacheAttnArgs)]
+    lib.pmkl_cache_attn_kernel_name.restype = ctypes.c_char_p
     _lib = lib
     return lib
 
@@ -267,3 +367,54 @@ def make_softmax_args(dst, src, *, out_dtype: int, in_dtype: int, elements: int,
     a.elements, a.stride, a.batch = elements, stride, batch
     a.is_log = 1 if is_log else 0
     return a
+
+
+def _fill(args, fields: dict):
+    for name, value in fields.items():
+        if isinstance(value, (tuple, list)):
+            getattr(args, name)[:] = [int(x) for x in value]
+        else:
+            setattr(args, name, value)
+    return args
+
+
+def make_kv_cache(k, v, k_scale, v_scale, **fields) -> KvCache:
+    """Build a KvCache from raw integer pointers, its sizes and, as tuples, strides."""
+    return _fill(KvCache(), dict(k=k, v=v, k_scale=k_scale, v_scale=v_scale, **fields))
+
+
+def make_cache_slots_args(**fields) -> CacheSlotsArgs:
+    """Build a CacheSlotsArgs; fields not given are zero."""
+    return _fill(CacheSlotsArgs(), fields)
+
+
+def make_cache_append_args(cache: KvCache, **fields) -> CacheAppendArgs:
+    """Build a CacheAppendArgs; fields not given are zero."""
+    return _fill(CacheAppendArgs(), dict(cache=cache, **fields))
+
+
+def make_cache_attn_args(cache: KvCache, **fields) -> CacheAttnArgs:
+    """Build a CacheAttnArgs; fields not given are zero."""
+    return _fill(CacheAttnArgs(), dict(cache=cache, **fields))
+
+
+def cache_slots_raw(args: CacheSlotsArgs, stream: int | None = None) -> int:
+    """Call pmkl_cache_slots; returns the status code."""
+    return load().pmkl_cache_slots(ctypes.byref(args), ctypes.c_void_p(stream or 0))
+
+
+def cache_append_raw(args: CacheAppendArgs, stream: int | None = None) -> int:
+    """Call pmkl_cache_append; returns the status code."""
+    return load().pmkl_cache_append(ctypes.byref(args), ctypes.c_void_p(stream or 0))
+
+
+def cache_attn_fwd_raw(args: CacheAttnArgs, stream: int | None = None) -> int:
+    """Call pmkl_cache_attn_fwd; returns the status code."""
+    return load().pmkl_cache_attn_fwd(ctypes.byref(args), ctypes.c_void_p(stream or 0))
+
+
+def cache_attn_kernel_name(args: CacheAttnArgs) -> str | None:
+    """The kernels (and launch shapes) pmkl_cache_attn_fwd would launch for args; None
+    where the call would fail (last_error() says why)."""
+    name = load().pmkl_cache_attn_kernel_name(ctypes.byref(args))
+    return None if name is None else name.decode()

@@ -29,6 +29,7 @@
 #include <limits>
 
 #include "../../include/pmkl_attn.h"
+#include "../../include/pmkl_cache.h"
 
 namespace {
 
@@ -391,6 +392,225 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> fused_self_attention_autograd(con
     return std::make_tuple(r[0], r[1], r[2]);
 }
 
+// The cache operators (pmkl_cache.h): device tensors only.  In native code as
+// their smallest calls take the card a few microseconds.
+namespace {
+
+void check_on(const char *op, const char *name, const at::Tensor &t, const at::Tensor &like, at::ScalarType type,
+              int64_t dim) {
+    TORCH_CHECK(t.device() == like.device(), op, ": ", name, " is on ", t.device(), ", not on ", like.device());
+    TORCH_CHECK(t.scalar_type() == type, op, ": ", name, " must be ", type, ", got ", t.scalar_type());
+    TORCH_CHECK(t.dim() == dim, op, ": ", name, " must have ", dim, " dimensions, got ", t.dim());
+}
+
+// Strides for the C ABI: the stride of a dimension of size 1 is never used and
+// may hold anything, so it is passed as 0.
+template <size_t N>
+void abi_strides(int64_t (&dst)[N], const at::Tensor &t) {
+    for (size_t i = 0; i < N; ++i) dst[i] = t.size(i) == 1 ? 0 : t.stride(i);
+}
+
+// Whether two positions share memory by a stride of 0: an expanded tensor.
+bool is_expanded(const at::Tensor &t) {
+    for (int64_t i = 0; i < t.dim(); ++i)
+        if (t.size(i) > 1 && t.stride(i) == 0) return true;
+    return false;
+}
+
+// [tokens, heads, head_dim] as the kernels can read it in place, or a copy.
+at::Tensor token_view(const at::Tensor &t) {
+    const int64_t vec = 16 / t.element_size();
+    bool ok = (t.stride(2) == 1 || t.size(2) == 1) && !is_expanded(t) &&
+              reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+    for (int i = 0; i < 2; ++i) ok = ok && (t.size(i) == 1 || t.stride(i) % vec == 0);
+    return ok ? t : t.contiguous();
+}
+
+pmkl_kv_cache cache_of(const char *op, const at::Tensor &like, const at::Tensor &k, const at::Tensor &v,
+                       const at::Tensor &k_scale, const at::Tensor &v_scale) {
+    check_on(op, "k_cache", k, like, at::kFloat8_e4m3fn, 4);
+    check_on(op, "v_cache", v, like, at::kFloat8_e4m3fn, 4);
+    check_on(op, "k_scale", k_scale, like, at::kFloat, 2);
+    check_on(op, "v_scale", v_scale, like, at::kFloat, 2);
+    TORCH_CHECK(v.size(0) == k.size(0) && v.size(1) == k.size(1) && v.size(2) == k.size(3) && v.size(3) == k.size(2),
+                op, ": k_cache is [pages, kv_heads, page_size, head_dim], v_cache [pages, kv_heads, head_dim, page_size]; got ",
+                k.sizes(), " and ", v.sizes());
+    for (const at::Tensor &s : {k_scale, v_scale})
+        TORCH_CHECK(s.size(0) == k.size(0) && s.size(1) == k.size(1), op,
+                    ": k_scale and v_scale must be [pages, kv_heads], got ", s.sizes());
+    TORCH_CHECK((k.stride(3) == 1 || k.size(3) == 1) && (v.stride(3) == 1 || v.size(3) == 1), op,
+                ": the last dimension of k_cache and v_cache must be contiguous");
+    TORCH_CHECK(!is_expanded(k) && !is_expanded(v) && !is_expanded(k_scale) && !is_expanded(v_scale), op,
+                ": the cache must not be expanded");
+    pmkl_kv_cache c;
+    std::memset(&c, 0, sizeof(c));
+    c.k = k.data_ptr();
+    c.v = v.data_ptr();
+    c.k_scale = static_cast<float *>(k_scale.data_ptr());
+    c.v_scale = static_cast<float *>(v_scale.data_ptr());
+    c.pages = k.size(0);
+    c.kv_heads = k.size(1);
+    c.page_size = k.size(2);
+    c.head_dim = k.size(3);
+    abi_strides(c.k_strides, k);
+    abi_strides(c.v_strides, v);
+    abi_strides(c.k_scale_strides, k_scale);
+    abi_strides(c.v_scale_strides, v_scale);
+    return c;
+}
+
+void *current_stream(const at::Tensor &t) {
+    return (void *)c10::hip::getCurrentHIPStream(t.device().index()).stream();
+}
+
+}  // namespace
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> cache_slots(const at::Tensor &cached_lens,
+                                                                       const at::Tensor &new_lens,
+                                                                       const at::Tensor &block_table,
+                                                                       const at::Tensor &free_pages,
+                                                                       const at::Tensor &free_head, int64_t page_size,
+                                                                       int64_t num_tokens) {
+    const char *op = "cache_slots";
+    TORCH_CHECK(cached_lens.is_cuda(), op, " takes ROCm device tensors");
+    check_on(op, "cached_lens", cached_lens, cached_lens, at::kInt, 1);
+    check_on(op, "new_lens", new_lens, cached_lens, at::kInt, 1);
+    check_on(op, "block_table", block_table, cached_lens, at::kInt, 2);
+    check_on(op, "free_pages", free_pages, cached_lens, at::kInt, 1);
+    check_on(op, "free_head", free_head, cached_lens, at::kInt, 1);
+    const int64_t B = cached_lens.size(0);
+    TORCH_CHECK(new_lens.size(0) == B && block_table.size(0) == B, op, ": cached_lens, new_lens and block_table must have ",
+                "one entry for each request");
+    TORCH_CHECK(free_head.size(0) == 1, op, ": free_head must have one element");
+    TORCH_CHECK(cached_lens.is_contiguous() && new_lens.is_contiguous() && free_pages.is_contiguous(), op,
+                ": cached_lens, new_lens and free_pages must be contiguous");
+    TORCH_CHECK(block_table.numel() == 0 || block_table.size(1) == 1 || block_table.stride(1) == 1, op, ": rows of block_table must be contiguous");
+    TORCH_CHECK(num_tokens >= 0, op, ": num_tokens must not be negative");
+    c10::OptionalDeviceGuard guard(cached_lens.device());
+    const auto ints = cached_lens.options();
+    auto seq_lens = at::empty({B}, ints), query_start = at::empty({B + 1}, ints), head = at::empty({1}, ints);
+    auto slots = at::empty({num_tokens}, ints.dtype(at::kLong));
+    pmkl_cache_slots_args a;
+    std::memset(&a, 0, sizeof(a));
+    a.cached_lens = static_cast<const int32_t *>(cached_lens.data_ptr());
+    a.new_lens = static_cast<const int32_t *>(new_lens.data_ptr());
+    a.block_table = static_cast<int32_t *>(block_table.data_ptr());
+    a.free_pages = static_cast<const int32_t *>(free_pages.data_ptr());
+    a.free_head = static_cast<const int32_t *>(free_head.data_ptr());
+    a.seq_lens = static_cast<int32_t *>(seq_lens.data_ptr());
+    a.query_start = static_cast<int32_t *>(query_start.data_ptr());
+    a.slots = static_cast<int64_t *>(slots.data_ptr());
+    a.free_head_out = static_cast<int32_t *>(head.data_ptr());
+    a.batch = B;
+    a.table_width = block_table.size(1);
+    a.table_stride = B > 1 && block_table.numel() > 0 ? block_table.stride(0) : 0;
+    TORCH_CHECK(B <= 1 || a.table_width == 0 || a.table_stride >= a.table_width, op, ": rows of block_table overlap");
+    a.free_count = free_pages.size(0);
+    a.page_size = page_size;
+    a.tokens = num_tokens;
+    const int rc = pmkl_cache_slots(&a, current_stream(cached_lens));
+    TORCH_CHECK(rc == PMKL_OK, op, ": ", pmkl_last_error());
+    return std::make_tuple(seq_lens, query_start, slots, head);
+}
+
+void cache_append(const at::Tensor &k, const at::Tensor &v, const at::Tensor &slots, const at::Tensor &k_cache,
+                  const at::Tensor &v_cache, const at::Tensor &k_scale, const at::Tensor &v_scale) {
+    const char *op = "cache_append";
+    TORCH_CHECK(k.is_cuda(), op, " takes ROCm device tensors");
+    const int32_t dt = to_pmkl_dtype(k.scalar_type());
+    TORCH_CHECK(dt >= 0, op, ": k and v must be float32, float16 or bfloat16, got ", k.scalar_type());
+    check_on(op, "k", k, k, k.scalar_type(), 3);
+    check_on(op, "v", v, k, k.scalar_type(), 3);
+    check_on(op, "slots", slots, k, at::kLong, 1);
+    pmkl_cache_append_args a;
+    std::memset(&a, 0, sizeof(a));
+    a.cache = cache_of(op, k, k_cache, v_cache, k_scale, v_scale);
+    TORCH_CHECK(k.sizes() == v.sizes() && k.size(1) == a.cache.kv_heads && k.size(2) == a.cache.head_dim, op,
+                ": k and v must be [tokens, ", a.cache.kv_heads, ", ", a.cache.head_dim, "], got ", k.sizes(), " and ",
+                v.sizes());
+    TORCH_CHECK(slots.size(0) == k.size(0) && slots.is_contiguous(), op, ": slots must be contiguous, one for each token");
+    if (k.numel() == 0) return;
+    c10::OptionalDeviceGuard guard(k.device());
+    auto kd = token_view(k), vd = token_view(v);
+    a.k = kd.data_ptr();
+    a.v = vd.data_ptr();
+    a.slots = static_cast<const int64_t *>(slots.data_ptr());
+    a.dtype = dt;
+    a.tokens = k.size(0);
+    abi_strides(a.k_strides, kd);
+    abi_strides(a.v_strides, vd);
+    const int rc = pmkl_cache_append(&a, current_stream(k));
+    TORCH_CHECK(rc == PMKL_OK, op, ": ", pmkl_last_error());
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> cache_attn_fwd(
+    const at::Tensor &q, const at::Tensor &k_cache, const at::Tensor &v_cache, const at::Tensor &k_scale,
+    const at::Tensor &v_scale, const at::Tensor &block_table, const at::Tensor &seq_lens, const at::Tensor &query_start,
+    bool is_causal, std::optional<double> scale, std::optional<at::Tensor> out, std::optional<at::Tensor> out_m,
+    std::optional<at::Tensor> out_l) {
+    const char *op = "cache_attn_fwd";
+    TORCH_CHECK(q.is_cuda(), op, " takes ROCm device tensors");
+    const int32_t dt = to_pmkl_dtype(q.scalar_type());
+    TORCH_CHECK(dt >= 0, op, ": q must be float32, float16 or bfloat16, got ", q.scalar_type());
+    check_on(op, "q", q, q, q.scalar_type(), 3);
+    pmkl_cache_attn_args a;
+    std::memset(&a, 0, sizeof(a));
+    a.cache = cache_of(op, q, k_cache, v_cache, k_scale, v_scale);
+    check_on(op, "block_table", block_table, q, at::kInt, 2);
+    check_on(op, "seq_lens", seq_lens, q, at::kInt, 1);
+    check_on(op, "query_start", query_start, q, at::kInt, 1);
+    const int64_t N = q.size(0), H = q.size(1), D = q.size(2), B = seq_lens.size(0);
+    TORCH_CHECK(D == a.cache.head_dim, op, ": head_dim of q is ", D, ", of the cache ", a.cache.head_dim);
+    TORCH_CHECK(block_table.size(0) == B && query_start.size(0) == B + 1, op,
+                ": block_table and query_start must have a row and a start for each of the ", B,
+                " requests, and query_start its end");
+    TORCH_CHECK(seq_lens.is_contiguous() && query_start.is_contiguous(), op,
+                ": seq_lens and query_start must be contiguous");
+    TORCH_CHECK(block_table.numel() == 0 || block_table.size(1) == 1 || block_table.stride(1) == 1, op, ": rows of block_table must be contiguous");
+    TORCH_CHECK(!scale.has_value() || *scale > 0, op, ": scale must be positive");
+    const auto result = [&](const char *name, const std::optional<at::Tensor> &given, at::IntArrayRef sizes,
+                            at::ScalarType type) {
+        if (!given.has_value()) return at::empty(sizes, q.options().dtype(type).memory_format(at::MemoryFormat::Contiguous));
+        check_on(op, name, *given, q, type, (int64_t)sizes.size());
+        TORCH_CHECK(given->sizes() == sizes, op, ": ", name, " must be ", sizes, ", got ", given->sizes());
+        return *given;
+    };
+    c10::OptionalDeviceGuard guard(q.device());
+    auto o = result("out", out, {N, H, D}, q.scalar_type());
+    auto m = result("out_m", out_m, {N, H}, at::kFloat), l = result("out_l", out_l, {N, H}, at::kFloat);
+    TORCH_CHECK(o.numel() == 0 || (o.stride(2) == 1 && !is_expanded(o)), op,
+                ": out must have a contiguous head_dim and not be expanded");
+    TORCH_CHECK(m.is_contiguous() && l.is_contiguous(), op, ": out_m and out_l must be contiguous");
+    auto qd = q.numel() ? token_view(q) : q;
+    a.q = qd.data_ptr();
+    a.o = o.data_ptr();
+    a.m = static_cast<float *>(m.data_ptr());
+    a.l = static_cast<float *>(l.data_ptr());
+    a.block_table = static_cast<const int32_t *>(block_table.data_ptr());
+    a.seq_lens = static_cast<const int32_t *>(seq_lens.data_ptr());
+    a.query_start = static_cast<const int32_t *>(query_start.data_ptr());
+    a.dtype = dt;
+    a.is_causal = is_causal ? 1 : 0;
+    a.scale = (float)scale.value_or(0.0);
+    a.tokens = N;
+    a.heads = H;
+    a.batch = B;
+    a.table_width = block_table.size(1);
+    a.table_stride = B > 1 && block_table.numel() > 0 ? block_table.stride(0) : 0;
+    TORCH_CHECK(B <= 1 || a.table_width == 0 || a.table_stride > 0, op, ": block_table must not be expanded");
+    abi_strides(a.q_strides, qd);
+    abi_strides(a.o_strides, o);
+    at::Tensor workspace;   // from torch's allocator: a captured graph has its own
+    if (const uint64_t bytes = pmkl_cache_attn_workspace_size(&a)) {
+        workspace = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+        a.workspace = workspace.data_ptr();
+        a.workspace_bytes = bytes;
+    }
+    const int rc = pmkl_cache_attn_fwd(&a, current_stream(q));
+    TORCH_CHECK(rc == PMKL_OK, op, ": ", pmkl_last_error());
+    return std::make_tuple(o, m, l);
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("fused_self_attention_fw", &fused_self_attention_fw, "fused_self_attention_fw",
           pybind11::arg("q"), pybind11::arg("k"), pybind11::arg("v"), pybind11::arg("is_causal"));
@@ -400,4 +620,15 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("fused_self_attention_autograd", &fused_self_attention_autograd,
           "fused_self_attention_fw with the backward recorded (device tensors)", pybind11::arg("q"),
           pybind11::arg("k"), pybind11::arg("v"), pybind11::arg("is_causal"));
+    m.def("cache_slots", &cache_slots, "block table entries and slots of a step's tokens", pybind11::arg("cached_lens"),
+          pybind11::arg("new_lens"), pybind11::arg("block_table"), pybind11::arg("free_pages"),
+          pybind11::arg("free_head"), pybind11::arg("page_size"), pybind11::arg("num_tokens"));
+    m.def("cache_append", &cache_append, "new keys and values into the cache", pybind11::arg("k"), pybind11::arg("v"),
+          pybind11::arg("slots"), pybind11::arg("k_cache"), pybind11::arg("v_cache"), pybind11::arg("k_scale"),
+          pybind11::arg("v_scale"));
+    m.def("cache_attn_fwd", &cache_attn_fwd, "attention over the cache", pybind11::arg("q"), pybind11::arg("k_cache"),
+          pybind11::arg("v_cache"), pybind11::arg("k_scale"), pybind11::arg("v_scale"), pybind11::arg("block_table"),
+          pybind11::arg("seq_lens"), pybind11::arg("query_start"), pybind11::arg("is_causal") = true,
+          pybind11::arg("scale") = pybind11::none(), pybind11::arg("out") = pybind11::none(),
+          pybind11::arg("out_m") = pybind11::none(), pybind11::arg("out_l") = pybind11::none());
 }
