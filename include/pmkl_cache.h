@@ -40,7 +40,8 @@ extern "C" {
 
 /* A cache.  Strides are in elements (bytes for the codes); a stride group that
  * is all zero means contiguous.  The codes' last dimension is contiguous, their
- * strides are multiples of 16 and their bases 16-byte aligned. */
+ * strides are multiples of 16 and their bases 16-byte aligned; pages lie less than
+ * 2 GiB apart. */
 typedef struct pmkl_kv_cache {
     void *k;                    /* [pages, kv_heads, page_size, head_dim] e4m3          */
     void *v;                    /* [pages, kv_heads, head_dim, page_size] e4m3          */
@@ -154,7 +155,9 @@ typedef struct pmkl_cache_attn_args {
  * fp32:
  *   s_j = scale * <q, key_j>,  m = max_j s_j,  l = sum_j exp(s_j - m),
  *   o   = sum_j exp(s_j - m) / l * value_j
- * The scales must be finite.  Tokens are hidden that lie past the
+ * The scales must be finite and not negative, and the v_scale of the pages that a row
+ * sees within 2^80 of each other (further down, values lose precision against the
+ * largest).  Tokens are hidden that lie past the
  * table's width or in a page whose table entry is outside 0 .. pages - 1 (whatever
  * the cache holds there); a row that sees none has o = 0, m = -inf, l = 0.  NaN in a
  * hidden token reaches nothing.  Rows of no request are not written.  query_start must

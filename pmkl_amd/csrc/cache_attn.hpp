@@ -1,26 +1,33 @@
 // gfx950 attention over the paged 8-bit cache (include/pmkl_cache.h).
 //
-// A workgroup owns 16 query rows of one request and key head: row r is query
-// head r % G of the head's G, token r / G, so that a key is read once for all
-// heads that share it.  Its waves take the request's tiles of 64 tokens in turn,
-// each with a running max, sum and output of its own, which the LDS joins at the
-// end.
+// The unit of work is a tile of 64 keys for 16 query rows of one request and key
+// head: row r is query head r % G of the head's G, token r / G, so that a key is
+// read once for all heads that share it.  A wave takes tiles one after the
+// other, with a running max, sum and output.  Which wave has which tiles, and
+// where they are joined: cache_attn_kernel, cache_split and cache_chunk below.
 //
 // Scores are formed transposed, S^T = K Q^T, and so is the output, O^T = V^T P^T,
-// with v_mfma_f32_16x16x32: codes become exact bf16 (f16 under f16 queries) on
-// the way from the load to the matrix unit, two in an instruction, and the
-// page's scale is a factor of the scores or probabilities.
-//   * Tile t of the four 16-key tiles has key 16 (i / 4) + 4 t + i % 4 in row i.
-//     Of the result a lane has rows 4 g .. 4 g + 3 (g = lane / 16), so over the
-//     four tiles it has the 16 consecutive keys 16 g ..: one page's, so one scale
-//     of the lane; and they are, in order, the lane's part of the P V product,
-//     whose V^T operand is 16 bytes of a column's tokens.  Nothing passes
-//     through the LDS or between lanes but the row max.
+// with v_mfma_f32_16x16x32: codes become exact 16-bit values on the way from the
+// load to the matrix unit, two in an instruction.
+//   * Of the four 16-key products of a tile, number t has key 16 (i / 4) + 4 t +
+//     i % 4 in row i.  Of the results a lane has rows 4 g .. 4 g + 3 (g = lane /
+//     16), so over the four it has the 16 consecutive keys 16 g ..: one page's, so
+//     one scale of the lane; and they are, in order, the lane's part of the P V
+//     product, whose V^T operand is 16 bytes of a column's tokens.  Nothing
+//     passes through the LDS or between lanes but the row max.
 //   * The contraction over columns may take them in any order, so a lane loads
 //     16 consecutive bytes of a key, two operands' worth.
-// fp32 queries are three bf16 terms (24 bits).  P is two bf16 terms, error 2^-17
-// (three under fp32 queries): with one, its 2^-9 would be as large as the
-// rounding of a bf16 output.
+//   * The next tile's keys are loaded when the scores have taken the registers
+//     of this one's, its values after P V, its table entries a tile earlier: 16
+//     KB (head_dim 128) of a wave are under way at any time.
+// Types.  Keys meet bf16 and fp32 queries in bf16 (the latter as three terms, 24
+// bits), f16 queries in f16.  P V is in f16: a weight times its page's scale is
+// (p m 2^14) (v 2^(e - E)) 2^(E - 14), with the scale m 2^e and the tile's largest
+// e as E.  The first factor is one f16 term under bf16 queries (error 2^-12 of a
+// weight, beside the output's 2^-9), two under the others (2^-22); the second is
+// exact, and free in the conversion, while e >= E - 14 (a tile whose scales lie
+// further apart takes another round for the larger ones); the third goes into the
+// factor that rescales the output anyway.
 #pragma once
 
 #include "cache_common.hpp"
@@ -33,6 +40,8 @@ typedef __bf16 cbf16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 cf16x8_t __attribute__((ext_vector_type(8)));
 typedef float cf32x4_t __attribute__((ext_vector_type(4)));
 
+struct CacheUnfinished;
+
 struct CacheAttnParams {
     const void *q;
     void *o;
@@ -42,6 +51,8 @@ struct CacheAttnParams {
     const int32_t *table;
     const int32_t *seq_lens;
     const int32_t *query_start;
+    float *parts;
+    CacheUnfinished *unfinished;
     int64_t q_st, q_sh, o_st, o_sh;   // elements
     int64_t table_stride;
     int32_t tokens;
@@ -51,15 +62,20 @@ struct CacheAttnParams {
     int32_t group;                    // query heads of a key head
     int32_t is_causal;
     float scale;
+    int32_t ranges;                   // of the split form
+    int32_t chunks;                   // whether chunks have their own workgroups
 };
 
-constexpr int kCacheTile = 64;   // keys
+constexpr int kCacheTile = 64;    // keys
+constexpr int kCacheRows = 16;    // query rows of a block
+constexpr int kPBits = 14;        // weights are held as p * 2^14
 
-// Queries of a type: how many terms, and the 16-bit type of the score product.
+// Queries of a type: the 16-bit type of the score product, how many terms a
+// query has there, and a weight in f16.
 template <typename T> struct CacheQuery;
 template <> struct CacheQuery<__bf16> {
     typedef cbf16x8_t frag;
-    static constexpr int QT = 1, PT = 2;
+    static constexpr int QT = 1, PT = 1;
 };
 template <> struct CacheQuery<_Float16> {
     typedef cf16x8_t frag;
@@ -67,7 +83,7 @@ template <> struct CacheQuery<_Float16> {
 };
 template <> struct CacheQuery<float> {
     typedef cbf16x8_t frag;
-    static constexpr int QT = 3, PT = 3;
+    static constexpr int QT = 3, PT = 2;
 };
 
 __device__ __forceinline__ cf32x4_t cache_mfma(cbf16x8_t a, cbf16x8_t b, cf32x4_t c) {
@@ -77,30 +93,34 @@ __device__ __forceinline__ cf32x4_t cache_mfma(cf16x8_t a, cf16x8_t b, cf32x4_t 
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// eight codes as an operand
+// eight codes as an operand, times a power of two
 template <typename F>
-__device__ __forceinline__ F cache_frag(uint32_t lo, uint32_t hi) {
+__device__ __forceinline__ F cache_frag(uint32_t lo, uint32_t hi, float scale = 1.f) {
     if constexpr (__is_same(F, cbf16x8_t)) {
-        const cbf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, false);
-        const cbf16x2_t b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, true);
-        const cbf16x2_t c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, false);
-        const cbf16x2_t d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, true);
+        const cbf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false);
+        const cbf16x2_t b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
+        const cbf16x2_t c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false);
+        const cbf16x2_t d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
         return F{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
     } else {
-        const cf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, false);
-        const cf16x2_t b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, true);
-        const cf16x2_t c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, false);
-        const cf16x2_t d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, true);
+        const cf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, scale, false);
+        const cf16x2_t b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, scale, true);
+        const cf16x2_t c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, scale, false);
+        const cf16x2_t d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, scale, true);
         return F{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
     }
 }
 
-// x as N bf16 terms, each the rounding of what those before leave
-template <int N>
-__device__ __forceinline__ void cache_terms(float x, __bf16 (&t)[N]) {
+// x as N terms of a 16-bit type, each the rounding of what those before leave.
+// Where x is a product, all terms must start from its fp32 value: contracted into
+// the subtraction and the conversions (v_fma_mix), the first term and the one that
+// is subtracted can round to different sides.
+template <int N, typename H>
+__device__ __forceinline__ void cache_terms(float x, H (&t)[N]) {
+    if constexpr (N > 1) asm("" : "+v"(x));
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        t[i] = (__bf16)x;
+        t[i] = (H)x;
         x -= (float)t[i];
     }
 }
@@ -110,74 +130,51 @@ __device__ __forceinline__ float cache_max(float a, float b) { return __builtin_
 // Whether a byte of x is the code of NaN (0x7f, 0xff): the high bit of each.
 __device__ __forceinline__ uint32_t cache_nan_bytes(uint32_t x) { return ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
-// A workgroup's rows.
+// Over the four 16-lane rows, of an integer that is the same in all lanes of a row.
+template <typename Op>
+__device__ __forceinline__ int cache_over_rows(int x, Op op) {
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = op((int)r[0], (int)r[1]);
+    const auto h = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return __builtin_amdgcn_readfirstlane(op((int)h[0], (int)h[1]));
+}
+
+// of a scale >= 0, -126 at least
+__device__ __forceinline__ int cache_exponent(float scale) { return max((int)(__float_as_uint(scale) >> 23 & 0xff), 1) - 127; }
+
+// A request's rows of one key head.
 struct CacheItem {
-    int b, head, row0;      // row0: first row of the tile, rows are token * group + head in the group
+    int b, head, row0;      // row0: the block's first row
     int q0, n;              // the request's first token, its tokens
     int length, keys;       // seq_len, and how many of its tokens the table holds
 };
 
 __device__ __forceinline__ CacheItem cache_request(const CacheAttnParams &p, int b) {
     CacheItem it;
-    it.b = b;
+    it.b = b, it.head = 0, it.row0 = 0;
     it.q0 = min(max(p.query_start[b], 0), p.tokens);
     it.n = min(max(p.query_start[b + 1], it.q0), p.tokens) - it.q0;
     it.length = max(p.seq_lens[b], 0);
-    it.keys = (int)min((int64_t)it.length, (int64_t)p.width << p.cache.log2_page);
+    it.keys = min(it.length, p.width << p.cache.log2_page);   // < 2^31 (checked)
     return it;
 }
 
-// keys that row t of the request's tokens sees
+// keys that the request's token t sees
 __device__ __forceinline__ int cache_limit(const CacheAttnParams &p, const CacheItem &it, int t) {
     return p.is_causal ? max(min(it.keys, it.length - it.n + t + 1), 0) : it.keys;
 }
 
-// The request and rows of work item i (tiles of R rows, then heads, then
-// requests): each wave sums the requests' tiles by itself.  False past the last.
-template <int R>
-__device__ __forceinline__ bool cache_find(const CacheAttnParams &p, int64_t i, int lane, CacheItem &it) {
-    int64_t sum = 0;
-    for (int base = 0; base < p.batch; base += 64) {
-        const int b = base + lane;
-        int64_t tiles = 0;
-        if (b < p.batch) {
-            const CacheItem r = cache_request(p, b);
-            tiles = ((int64_t)r.n * p.group + R - 1) / R * p.kv_heads;
-        }
-        const int64_t end = wave_scan(tiles, lane) + sum;
-        const uint64_t mask = __builtin_amdgcn_ballot_w64(i < end);
-        if (mask) {
-            const int l = __builtin_ctzll(mask);
-            it = cache_request(p, base + l);
-            const int64_t rem = i - (__shfl(end, l) - __shfl(tiles, l));
-            const int per_head = (int)(__shfl(tiles, l) / p.kv_heads);
-            it.head = (int)(rem / per_head);
-            it.row0 = (int)(rem % per_head) * R;
-            return true;
-        }
-        sum = __shfl(end, 63);
-    }
-    return false;
+__device__ __forceinline__ int64_t cache_rows(const CacheAttnParams &p, const CacheItem &it) {
+    return (int64_t)it.n * p.group;
 }
+__device__ __forceinline__ int cache_blocks(const CacheAttnParams &p, const CacheItem &it) {   // of 16 rows
+    return (int)((cache_rows(p, it) + kCacheRows - 1) / kCacheRows);
+}
+// tiles that a row block of the request counts for: its keys' (one at least, so
+// that rows that see nothing are written)
+__device__ __forceinline__ int cache_tiles(const CacheItem &it) { return max((it.keys + kCacheTile - 1) / kCacheTile, 1); }
 
-// NW waves; 16 rows of the workgroup.
-template <typename T, int D, int NW>
-__global__ __launch_bounds__(NW * 64) void cache_attn_kernel(CacheAttnParams p) {
-    using CQ = CacheQuery<T>;
-    typedef typename CQ::frag frag;
-    constexpr int QT = CQ::QT, PT = CQ::PT;
-    constexpr int R = 16;
-    constexpr int NK = D / 32;          // operands of a key
-    constexpr int NB = D / 16;          // 16-column blocks of the output
-    constexpr int LD = D + 4;           // row of the LDS
-    constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
-    __shared__ __attribute__((aligned(16))) float part[NW][R][LD];
-    __shared__ float part_m[NW][R], part_l[NW][R];
-
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int g = lane >> 4, r16 = lane & 15;
-    CacheItem it;
-    if (!cache_find<R>(p, blockIdx.x, lane, it)) return;
+__device__ __forceinline__ void cache_uniform(CacheItem &it) {
     it.b = __builtin_amdgcn_readfirstlane(it.b);
     it.head = __builtin_amdgcn_readfirstlane(it.head);
     it.row0 = __builtin_amdgcn_readfirstlane(it.row0);
@@ -185,218 +182,823 @@ __global__ __launch_bounds__(NW * 64) void cache_attn_kernel(CacheAttnParams p) 
     it.n = __builtin_amdgcn_readfirstlane(it.n);
     it.length = __builtin_amdgcn_readfirstlane(it.length);
     it.keys = __builtin_amdgcn_readfirstlane(it.keys);
-    const int64_t rows = (int64_t)it.n * p.group;   // < 2^31 (checked)
+}
 
-    // this lane's row, and its query as operands
-    const int row = it.row0 + r16;
-    const bool live = row < rows;
-    const int token = live ? row / p.group : 0;
-    const int limit = live ? cache_limit(p, it, token) : 0;
-    frag q[QT][NK];
-    {
-        const T *src = (const T *)p.q + (int64_t)(it.q0 + token) * p.q_st + (int64_t)(it.head * p.group + (live ? row % p.group : 0)) * p.q_sh;
+// Requests in order have weight(request) units each (fewer than 2^31 in all:
+// checked); finds the one with unit i, and i counted from its first.  Every wave
+// sums by itself, 64 requests at a time.  False past the last unit.
+template <typename Weight>
+__device__ __forceinline__ bool cache_find(const CacheAttnParams &p, int &i, int lane, CacheItem &it, Weight weight) {
+    for (int base = 0; base < p.batch; base += 64) {
+        const int b = base + lane;
+        const int own = b < p.batch ? weight(cache_request(p, b)) : 0;
+        const int end = wave_scan(own);
+        const uint64_t mask = __builtin_amdgcn_ballot_w64(i < end);
+        if (mask) {
+            const int l = __builtin_ctzll(mask);
+            i -= __builtin_amdgcn_readlane(end, l) - __builtin_amdgcn_readlane(own, l);
+            it = cache_request(p, base + l);
+            return true;
+        }
+        i -= __builtin_amdgcn_readlane(end, 63);
+    }
+    return false;
+}
+template <typename Weight>
+__device__ __forceinline__ int cache_total(const CacheAttnParams &p, int lane, Weight weight) {
+    int sum = 0;
+    for (int b = lane; b < p.batch; b += 64) sum += weight(cache_request(p, b));
+    return __builtin_amdgcn_readlane(wave_scan(sum), 63);
+}
+
+// A head's pages.  Strides between pages are below 2^31 (checked): a page's place
+// is one multiply-add.
+struct CacheHead {
+    const uint8_t *k, *v;
+    const char *ks, *vs;
+    const int32_t *table;   // the request's row
+    int last_page;
+
+    __device__ __forceinline__ CacheHead(const CacheAttnParams &p, const CacheItem &it) {
+        k = p.cache.k + (int64_t)it.head * p.cache.k_sh;
+        v = p.cache.v + (int64_t)it.head * p.cache.v_sh;
+        ks = (const char *)(p.cache.k_scale + (int64_t)it.head * p.cache.ks_sh);
+        vs = (const char *)(p.cache.v_scale + (int64_t)it.head * p.cache.vs_sh);
+        table = p.table + (int64_t)it.b * p.table_stride;
+        last_page = (it.keys - 1) >> p.cache.log2_page;
+    }
+    // table entry of the page of a key
+    __device__ __forceinline__ int entry(const CacheAttnParams &p, int key) const {
+        return table[(uint32_t)min(key >> p.cache.log2_page, last_page)];
+    }
+};
+__device__ __forceinline__ uint32_t cache_page(const CacheAttnParams &p, int entry) {
+    return (uint32_t)entry < (uint32_t)p.cache.pages ? entry : 0;
+}
+template <typename T>
+__device__ __forceinline__ const T *cache_at(const T *base, uint32_t page, uint32_t stride) { return base + (uint64_t)page * stride; }
+
+// Two dwords: eight codes.
+struct CacheCodes { uint32_t lo, hi; };
+
+// A wave's rows: QB blocks of 16, of one request and key head, a column of the
+// results each.
+template <typename T, int D, int QB>
+struct CacheRows {
+    using CQ = CacheQuery<T>;
+    typedef typename CQ::frag frag;
+    static constexpr int QT = CQ::QT, PT = CQ::PT;
+    static constexpr int NK = D / 32;          // operands of a key
+    static constexpr int NB = D / 16;          // 16-column blocks of the output
+
+    frag q[QB][QT][NK];
+    cf32x4_t o[QB][NB];     // sum p v, in units of 2^(unit - 14) (relative to m)
+    float m[QB], l[QB];     // m in units of log2; l of this lane's keys
+    int limit[QB];          // keys that the lane's row sees
+    int first_limit, last_limit;   // that the wave's first and last row see
+    int unit, peak;
+    uint32_t nans;          // what masked tiles had to clear
+
+    // rows it.row0 + 16 b + column, as operands
+    __device__ __forceinline__ void load(const CacheAttnParams &p, const CacheItem &it, int lane) {
+        const int g = lane >> 4;
+        const int64_t rows = cache_rows(p, it);
 #pragma unroll
-        for (int k = 0; k < NK; ++k) {
-            const int d = D >= 64 ? k / 2 * 64 + g * 16 + k % 2 * 8 : g * 8;
-            struct alignas(16) { T v[8]; } x{};
-            if (live) x = *(const decltype(x) *)(src + d);
+        for (int b = 0; b < QB; ++b) {
+            const int64_t row = (int64_t)it.row0 + b * kCacheRows + (lane & 15);
+            const bool live = row < rows;
+            const int token = live ? (int)row / p.group : 0;
+            limit[b] = live ? cache_limit(p, it, token) : 0;
+            const T *src = (const T *)p.q + (int64_t)(it.q0 + token) * p.q_st + (int64_t)(it.head * p.group + (live ? (int)row % p.group : 0)) * p.q_sh;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                if constexpr (QT == 1) {
-                    q[0][k][e] = x.v[e];
-                } else {
-                    __bf16 t[QT];
-                    cache_terms<QT>((float)x.v[e], t);
+            for (int k = 0; k < NK; ++k) {
+                const int d = D >= 64 ? k / 2 * 64 + g * 16 + k % 2 * 8 : g * 8;
+                struct alignas(16) { T v[8]; } x{};
+                if (live) x = *(const decltype(x) *)(src + d);
 #pragma unroll
-                    for (int i = 0; i < QT; ++i) q[i][k][e] = t[i];
+                for (int e = 0; e < 8; ++e) {
+                    if constexpr (QT == 1) {
+                        q[b][0][k][e] = x.v[e];
+                    } else {
+                        __bf16 t[QT];
+                        cache_terms<QT>((float)x.v[e], t);
+#pragma unroll
+                        for (int i = 0; i < QT; ++i) q[b][i][k][e] = t[i];
+                    }
                 }
+            }
+#pragma unroll
+            for (int i = 0; i < NB; ++i) o[b][i] = cf32x4_t{};
+            m[b] = -INFINITY, l[b] = 0.f;
+        }
+        unit = peak = -126;
+        nans = 0;
+        first_limit = it.row0 < rows ? cache_limit(p, it, it.row0 / p.group) : 0;
+        last_limit = last_key(p, it);
+    }
+    // keys that the last of the rows sees
+    static __device__ __forceinline__ int last_key(const CacheAttnParams &p, const CacheItem &it) {
+        const int64_t rows = cache_rows(p, it);
+        return it.row0 < rows ? cache_limit(p, it, (int)(min((int64_t)it.row0 + QB * kCacheRows, rows) - 1) / p.group) : 0;
+    }
+
+    template <typename K>
+    __device__ __forceinline__ void scores(cf32x4_t (&s)[QB][4], K keys) const {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+#pragma unroll
+            for (int b = 0; b < QB; ++b) s[b][t] = cf32x4_t{};
+#pragma unroll
+            for (int k = 0; k < NK; ++k) {
+                const CacheCodes x = keys(t, k);
+                const frag a = cache_frag<frag>(x.lo, x.hi);
+#pragma unroll
+                for (int i = QT - 1; i >= 0; --i)    // the smallest first
+#pragma unroll
+                    for (int b = 0; b < QB; ++b) s[b][t] = cache_mfma(a, q[b][i][k], s[b][t]);
             }
         }
     }
-    // what the tile's first and last row see
-    const int first_limit = cache_limit(p, it, it.row0 / p.group);
-    const int last_limit = cache_limit(p, it, (int)(min((int64_t)it.row0 + R, rows) - 1) / p.group);
-    const int tiles = (last_limit + kCacheTile - 1) / kCacheTile;
 
-    const uint8_t *kbase = p.cache.k + (int64_t)it.head * p.cache.k_sh;
-    const uint8_t *vbase = p.cache.v + (int64_t)it.head * p.cache.v_sh;
-    const float *ksbase = p.cache.k_scale + (int64_t)it.head * p.cache.ks_sh;
-    const float *vsbase = p.cache.v_scale + (int64_t)it.head * p.cache.vs_sh;
-    const int32_t *table = p.table + (int64_t)it.b * p.table_stride;
-    const int in_page = (1 << p.cache.log2_page) - 1;
-    const float c0 = p.scale * kLog2e;
-
-    cf32x4_t o[NB];
+    // Scores (times c) to weights; alpha: what the sums so far are worth now.
+    __device__ __forceinline__ void weigh(cf32x4_t (&s)[QB][4], float c, float (&alpha)[QB]) {
 #pragma unroll
-    for (int i = 0; i < NB; ++i) o[i] = cf32x4_t{};
-    float m = -INFINITY, l = 0.f;       // in units of log2; l of this lane's keys
-
-    for (int tile = wave; tile < tiles; tile += NW) {
-        const int key0 = tile * kCacheTile;
-        // the page of the rows that the lane loads, and of the keys it owns
-        const int kkey = key0 + (r16 >> 2) * 16, vkey = key0 + g * 16;
-        const int last_page = (it.keys - 1) >> p.cache.log2_page;
-        const int kentry = table[min(kkey >> p.cache.log2_page, last_page)];
-        const int ventry = table[min(vkey >> p.cache.log2_page, last_page)];
-        const bool held = (uint32_t)ventry < (uint32_t)p.cache.pages && vkey < it.keys;
-        const int64_t kpage = (uint32_t)kentry < (uint32_t)p.cache.pages ? kentry : 0;
-        const int64_t vpage = (uint32_t)ventry < (uint32_t)p.cache.pages ? ventry : 0;
-
-        const float ks = ksbase[vpage * p.cache.ks_sp], vs = vsbase[vpage * p.cache.vs_sp];
-        const uint8_t *kp = kbase + kpage * p.cache.k_sp + (int64_t)((kkey & in_page) + (r16 & 3)) * p.cache.k_st;
-        const uint8_t *vp = vbase + vpage * p.cache.v_sp + (vkey & in_page) + (int64_t)r16 * p.cache.v_sd;
-
-        uint32_t kr[4][2 * NK], vr[NB][4];
+        for (int b = 0; b < QB; ++b) {
+            float mx = s[b][0][0];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            const uint8_t *kt = kp + t * 4 * p.cache.k_st;
-            if constexpr (D >= 64) {
+            for (int e = 1; e < 16; ++e) mx = cache_max(mx, s[b][e / 4][e % 4]);
+            mx = cache_max(m[b], across_rows(mx * c, [](float a, float b) { return cache_max(a, b); }));
+            const float ref = mx == -INFINITY ? 0.f : mx;
+            alpha[b] = __builtin_amdgcn_exp2f(m[b] - ref);
+            m[b] = mx;
+            float sum = 0.f;
 #pragma unroll
-                for (int c = 0; c < D / 64; ++c) {
-                    const uint4 x = *(const uint4 *)(kt + c * 64 + g * 16);
-                    kr[t][4 * c] = x.x, kr[t][4 * c + 1] = x.y, kr[t][4 * c + 2] = x.z, kr[t][4 * c + 3] = x.w;
-                }
-            } else {
-                const uint2 x = *(const uint2 *)(kt + g * 8);
-                kr[t][0] = x.x, kr[t][1] = x.y;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < NB; ++i) {
-            const uint4 x = *(const uint4 *)(vp + (int64_t)i * 16 * p.cache.v_sd);
-            vr[i][0] = x.x, vr[i][1] = x.y, vr[i][2] = x.z, vr[i][3] = x.w;
-        }
-
-        cf32x4_t s[4];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            s[t] = cf32x4_t{};
-#pragma unroll
-            for (int k = 0; k < NK; ++k) {
-                const frag a = cache_frag<frag>(kr[t][2 * k], kr[t][2 * k + 1]);
-#pragma unroll
-                for (int i = QT - 1; i >= 0; --i) s[t] = cache_mfma(a, q[i][k], s[t]);   // the smallest first
-            }
-        }
-        const float c = c0 * ks;
-        const bool masked = key0 + kCacheTile > first_limit || __builtin_amdgcn_ballot_w64(!held) != 0;
-        const int seen = held ? limit - vkey : 0;     // of the lane's 16 keys, those below are visible
-        float mx = -INFINITY;
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                s[t][e] *= c;
-                if (masked && 4 * t + e >= seen) s[t][e] = -INFINITY;
-                mx = cache_max(mx, s[t][e]);
-            }
-        mx = cache_max(m, across_rows(mx, [](float a, float b) { return cache_max(a, b); }));
-        const float ref = mx == -INFINITY ? 0.f : mx;
-        const float alpha = __builtin_amdgcn_exp2f(m - ref);
-        m = mx;
-        cbf16x8_t ph[PT][2];
-        float sum = 0.f;
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float x = __builtin_amdgcn_exp2f(s[t][e] - ref);
+            for (int e = 0; e < 16; ++e) {
+                const float x = __builtin_amdgcn_exp2f(fmaf(s[b][e / 4][e % 4], c, -ref));
+                s[b][e / 4][e % 4] = x;
                 sum += x;
-                float y = x * vs;
-                if (masked && 4 * t + e >= seen) y = 0.f;
-                __bf16 terms[PT];
-                cache_terms<PT>(y, terms);
-#pragma unroll
-                for (int i = 0; i < PT; ++i) ph[i][t / 2][t % 2 * 4 + e] = terms[i];
             }
-        l = l * alpha + sum;
-#pragma unroll
-        for (int i = 0; i < NB; ++i) o[i] *= alpha;
-
-        if (masked) {
-            // Hidden values count for nothing, also where they are NaN: what no
-            // row sees is cleared, a NaN that some rows see becomes 0 and is
-            // put into these rows' outputs.
-            uint32_t nans = 0;
-#pragma unroll
-            for (int i = 0; i < NB; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int n = held ? min(max(last_limit - vkey - 4 * j, 0), 4) : 0;
-                    vr[i][j] &= n ? 0xffffffffu >> (32 - 8 * n) : 0u;
-                    nans |= cache_nan_bytes(vr[i][j]);
-                }
-            if (__builtin_amdgcn_ballot_w64(nans != 0)) {
-                cbf16x8_t see[2];
-#pragma unroll
-                for (int e = 0; e < 16; ++e) see[e / 8][e % 8] = (__bf16)(e < seen ? 1.f : 0.f);
-#pragma unroll
-                for (int i = 0; i < NB; ++i) {
-                    cf32x4_t hit{};
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        cbf16x8_t bad;
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            const uint32_t f = cache_nan_bytes(vr[i][2 * h + j]);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) bad[4 * j + e] = (__bf16)(f >> (8 * e + 7) & 1 ? 1.f : 0.f);
-                            vr[i][2 * h + j] &= ~((f >> 7) * 0xffu);
-                        }
-                        hit = cache_mfma(bad, see[h], hit);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (hit[e] > 0.f) o[i][e] = __builtin_nanf("");
-                }
-            }
+            l[b] = l[b] * alpha[b] + sum;
         }
+    }
+
+    // A tile that every row sees whole, of pages of the cache whose scales lie
+    // within 2^14 (their exponents' largest is `now`): nearly all tiles.
+    // keys(t, k) and values(i, h) give the operands' codes; taken() is called
+    // when the keys have been taken.
+    template <typename K, typename V, typename F>
+    __device__ __forceinline__ void step(float c, float vs, int exponent, int now, K keys, V values, F taken) {
+        cf32x4_t s[QB][4];
+        float alpha[QB];
+        scores(s, keys);
+        taken();
+        weigh(s, c, alpha);
+        const float weight = __builtin_amdgcn_ldexpf(vs, kPBits - exponent), vscale = __builtin_amdgcn_ldexpf(1.f, exponent - now);
+        cf16x8_t ph[QB][PT][2];
+#pragma unroll
+        for (int b = 0; b < QB; ++b) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                _Float16 terms[PT];
+                cache_terms<PT>(s[b][e / 4][e % 4] * weight, terms);
+#pragma unroll
+                for (int i = 0; i < PT; ++i) ph[b][i][e / 8][e % 8] = terms[i];
+            }
+            const float rescale = __builtin_amdgcn_ldexpf(alpha[b], unit - now);
+#pragma unroll
+            for (int i = 0; i < NB; ++i) o[b][i] *= rescale;
+        }
+        unit = now;
+        peak = max(peak, now);
 #pragma unroll
         for (int i = 0; i < NB; ++i)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const cbf16x8_t a = cache_frag<cbf16x8_t>(vr[i][2 * h], vr[i][2 * h + 1]);
+                const CacheCodes x = values(i, h);
+                const cf16x8_t a = cache_frag<cf16x8_t>(x.lo, x.hi, vscale);
 #pragma unroll
-                for (int j = PT - 1; j >= 0; --j) o[i] = cache_mfma(a, ph[j][h], o[i]);
+                for (int j = PT - 1; j >= 0; --j)
+#pragma unroll
+                    for (int b = 0; b < QB; ++b) o[b][i] = cache_mfma(a, ph[b][j][h], o[b][i]);
             }
     }
 
-    // Join the waves.
-    l = across_rows(l, [](float a, float b) { return a + b; });
+    // Any other tile; its lane has keys vkey .. vkey + 15, `held` if their page is
+    // one of the cache's.
+    template <typename K, typename V, typename F>
+    __device__ __forceinline__ void step_any(int vkey, bool held, float c, float vs, K keys, V values, F taken) {
+        cf32x4_t s[QB][4];
+        float alpha[QB];
+        scores(s, keys);
+        taken();
 #pragma unroll
-    for (int i = 0; i < NB; ++i) *(cf32x4_t *)&part[wave][r16][i * 16 + g * 4] = o[i];
-    if (g == 0) {
-        part_m[wave][r16] = m;
-        part_l[wave][r16] = l;
+        for (int b = 0; b < QB; ++b) {
+            const int seen = held ? limit[b] - vkey : 0;   // of the lane's 16 keys, those below are visible
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float x = s[b][e / 4][e % 4] * c;
+                s[b][e / 4][e % 4] = e < seen ? x : -INFINITY;
+            }
+        }
+        weigh(s, 1.f, alpha);
+        // Hidden values count for nothing, also where they are NaN: what no row of
+        // the wave sees is cleared, and a NaN that some see is 0 here and put into
+        // these rows' outputs in the end.
+        uint32_t clear[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int n = held ? min(max(last_limit - vkey - 4 * j, 0), 4) : 0;
+            clear[j] = n ? 0xffffffffu >> (32 - 8 * n) : 0u;
+        }
+        // Pages within 2^14 of the least scale take part together, then the others.
+        const float scale = held ? vs : 0.f;
+        const int exponent = cache_exponent(scale);
+        bool todo = held;
+        while (__builtin_amdgcn_ballot_w64(todo) != 0) {    // (no page: alpha is 1, or there is nothing yet)
+            const int least = cache_over_rows(todo ? exponent : 128, [](int a, int b) { return min(a, b); });
+            const bool use = todo && exponent <= least + kPBits;
+            // (what is summed must not overflow: the unit stays within 2^80 of its highest)
+            const int now = max(cache_over_rows(use ? exponent : -126, [](int a, int b) { return max(a, b); }), peak - 80);
+            const float weight = use ? __builtin_amdgcn_ldexpf(scale, kPBits - exponent) : 0.f;
+            const float vscale = __builtin_amdgcn_ldexpf(1.f, use ? exponent - now : 0);
+            cf16x8_t ph[QB][PT][2];
+#pragma unroll
+            for (int b = 0; b < QB; ++b) {
+                const int seen = held ? limit[b] - vkey : 0;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    // (the weight of a page that the row does not see may be anything)
+                    const float x = e < seen ? s[b][e / 4][e % 4] * weight : 0.f;
+                    _Float16 terms[PT];
+                    cache_terms<PT>(x, terms);
+#pragma unroll
+                    for (int i = 0; i < PT; ++i) ph[b][i][e / 8][e % 8] = terms[i];
+                }
+                const float rescale = __builtin_amdgcn_ldexpf(alpha[b], unit - now);
+                alpha[b] = 1.f;
+#pragma unroll
+                for (int i = 0; i < NB; ++i) o[b][i] *= rescale;
+            }
+            unit = now;
+            peak = max(peak, now);
+            todo = todo && !use;
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const CacheCodes x = values(i, h);
+                    const uint32_t lo = x.lo & clear[2 * h], hi = x.hi & clear[2 * h + 1];
+                    const uint32_t bad = cache_nan_bytes(lo), bad2 = cache_nan_bytes(hi);
+                    nans |= bad | bad2;
+                    const cf16x8_t a = cache_frag<cf16x8_t>(lo & ~(bad | (bad - (bad >> 7))), hi & ~(bad2 | (bad2 - (bad2 >> 7))), vscale);
+#pragma unroll
+                    for (int j = PT - 1; j >= 0; --j)
+#pragma unroll
+                        for (int b = 0; b < QB; ++b) o[b][i] = cache_mfma(a, ph[b][j][h], o[b][i]);
+                }
+        }
     }
-    __syncthreads();
-    for (int i = tid; i < R * D / 4; i += NW * 64) {
-        const int r = i / (D / 4), d = i % (D / 4) * 4;
-        if (it.row0 + r >= rows) continue;
-        float mx = part_m[0][r];
+
+    // Whether step() does for a tile, and its largest exponent.
+    __device__ __forceinline__ bool whole(int key0, bool held, int exponent, int &now) const {
+        now = cache_over_rows(exponent, [](int a, int b) { return max(a, b); });
+        return key0 + kCacheTile <= first_limit && now >= peak - 80 &&
+               __builtin_amdgcn_ballot_w64(!held || exponent < now - kPBits) == 0;
+    }
+
+    // After the tiles tile, tile + step, ... below end: o in units of 1, l of the row,
+    // and NaN to the outputs of the rows that see a NaN value of a masked tile.
+    __device__ __forceinline__ void finish(const CacheAttnParams &p, const CacheItem &it, int tile, int end, int step, int lane) {
 #pragma unroll
-        for (int w = 1; w < NW; ++w) mx = cache_max(mx, part_m[w][r]);
+        for (int b = 0; b < QB; ++b) {
+            l[b] = across_rows(l[b], [](float a, float b) { return a + b; });
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[b][i][e] = __builtin_amdgcn_ldexpf(o[b][i][e], unit - kPBits);
+        }
+        if (__builtin_amdgcn_ballot_w64(nans != 0) == 0) return;
+        const int g = lane >> 4, r16 = lane & 15, in_page = (1 << p.cache.log2_page) - 1;
+        const CacheHead head(p, it);
+        for (; tile < end; tile += step) {
+            const int key0 = tile * kCacheTile, vkey = key0 + g * 16;
+            const int entry = head.entry(p, vkey);
+            const bool held = (uint32_t)entry < (uint32_t)p.cache.pages && vkey < it.keys;
+            if (key0 + kCacheTile <= first_limit && __builtin_amdgcn_ballot_w64(!held) == 0) continue;
+            const uint8_t *vp = cache_at(head.v, held ? entry : 0, p.cache.v_sp) + (vkey & in_page) + (int64_t)r16 * p.cache.v_sd;
+            const int any = held ? last_limit - vkey : 0;
+#pragma unroll
+            for (int i = 0; i < NB; ++i) {
+                const uint4 x = *(const uint4 *)(vp + (int64_t)i * 16 * p.cache.v_sd);
+                const uint32_t v[4] = {x.x, x.y, x.z, x.w};
+                cbf16x8_t bad[2];
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    bad[e / 8][e % 8] = (__bf16)((cache_nan_bytes(v[e / 4]) >> (8 * (e % 4) + 7) & 1) && e < any ? 1.f : 0.f);
+#pragma unroll
+                for (int b = 0; b < QB; ++b) {
+                    const int seen = held ? limit[b] - vkey : 0;
+                    cf32x4_t hit{};
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        cbf16x8_t see;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) see[e] = (__bf16)(8 * h + e < seen ? 1.f : 0.f);
+                        hit = cache_mfma(bad[h], see, hit);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (hit[e] > 0.f) o[b][i][e] = __builtin_nanf("");
+                }
+            }
+        }
+    }
+};
+
+// NT: past the caches' usual policy (nontemporal), for tiles that are read once. On
+// 1 GiB of scattered 2 KB pages, read by 512 workgroups, 6.7 TB/s against 5.9; but
+// chunks whose 32 row blocks share the tiles 670 us against 423.
+template <bool NT, typename V>
+__device__ __forceinline__ V cache_load(const uint8_t *p) {
+    typedef uint32_t words __attribute__((ext_vector_type(sizeof(V) / 4)));
+    return __builtin_bit_cast(V, NT ? __builtin_nontemporal_load((const words *)p) : *(const words *)p);
+}
+
+// 16 rows whose tiles the wave loads into registers.
+template <typename T, int D>
+struct CacheWave : CacheRows<T, D, 1> {
+    using Rows = CacheRows<T, D, 1>;
+    static constexpr int NK = Rows::NK, NB = Rows::NB;
+    uint32_t kr[4][2 * NK], vr[NB][4];
+    float ks, vs;
+
+    // kp, vp: the lane's part of a page (below)
+    template <bool NT>
+    __device__ __forceinline__ void load_keys(const CacheAttnParams &p, const CacheHead &head, const uint8_t *kp, int tile, int kentry, int ventry) {
+        const uint8_t *kt = cache_at(kp, cache_page(p, kentry), p.cache.k_sp) + (tile * kCacheTile & (1 << p.cache.log2_page) - 1) * p.cache.k_st;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            if constexpr (D >= 64) {
+#pragma unroll
+                for (int c = 0; c < D / 64; ++c) {
+                    const uint4 x = cache_load<NT, uint4>(kt + c * 64);
+                    kr[t][4 * c] = x.x, kr[t][4 * c + 1] = x.y, kr[t][4 * c + 2] = x.z, kr[t][4 * c + 3] = x.w;
+                }
+            } else {
+                const uint2 x = cache_load<NT, uint2>(kt);
+                kr[t][0] = x.x, kr[t][1] = x.y;
+            }
+            kt += 4 * p.cache.k_st;
+        }
+        const uint32_t page = cache_page(p, ventry);
+        ks = *(const float *)cache_at(head.ks, page, p.cache.ks_sp);
+        vs = *(const float *)cache_at(head.vs, page, p.cache.vs_sp);
+    }
+    template <bool NT>
+    __device__ __forceinline__ void load_values(const CacheAttnParams &p, const uint8_t *vp, int tile, int ventry) {
+        vp = cache_at(vp, cache_page(p, ventry), p.cache.v_sp) + (tile * kCacheTile & (1 << p.cache.log2_page) - 1);
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            const uint4 x = cache_load<NT, uint4>(vp);
+            vr[i][0] = x.x, vr[i][1] = x.y, vr[i][2] = x.z, vr[i][3] = x.w;
+            vp += 16 * p.cache.v_sd;
+        }
+    }
+
+    // Tiles tile, tile + step, ... below end.
+    __device__ __forceinline__ void run(const CacheAttnParams &p, const CacheItem &it, int tile, int end, int step, int lane) {
+        if (cache_blocks(p, it) == 1)
+            tiles<true>(p, it, tile, end, step, lane);
+        else
+            tiles<false>(p, it, tile, end, step, lane);
+    }
+    template <bool NT>
+    __device__ __forceinline__ void tiles(const CacheAttnParams &p, const CacheItem &it, int tile, int end, int step, int lane) {
+        const int g = lane >> 4, r16 = lane & 15, in_page = (1 << p.cache.log2_page) - 1;
+        end = min(end, (this->last_key(p, it) + kCacheTile - 1) / kCacheTile);
+        if (tile >= end) {
+            this->load(p, it, lane);
+            return;
+        }
+        const int begin = tile;
+        const CacheHead head(p, it);
+        // key 16 (r16 / 4) + r16 % 4 of a tile, columns 16 g ..; column r16, key 16 g
+        const uint8_t *kp = head.k + (int64_t)((r16 >> 2) * 16 & in_page) * p.cache.k_st + (r16 & 3) * p.cache.k_st + g * (D >= 64 ? 16 : 8);
+        const uint8_t *vp = head.v + (g * 16 & in_page) + (int64_t)r16 * p.cache.v_sd;
+        const auto entry = [&](int tile, int block) { return head.entry(p, tile * kCacheTile + block * 16); };
+        int kentry = entry(tile, r16 >> 2), ventry = entry(tile, g);
+        const int next = min(tile + step, end - 1);
+        int knext = entry(next, r16 >> 2), vnext = entry(next, g);
+        this->load(p, it, lane);
+        load_keys<NT>(p, head, kp, tile, kentry, ventry);
+        load_values<NT>(p, vp, tile, ventry);
+        const float c0 = p.scale * 1.44269504088896341f;
+        const auto keys = [&](int t, int k) { return CacheCodes{kr[t][2 * k], kr[t][2 * k + 1]}; };
+        const auto values = [&](int i, int h) { return CacheCodes{vr[i][2 * h], vr[i][2 * h + 1]}; };
+        // Whole tiles as long as there are such, then the others.
+        bool any = false;
+        for (; tile < end; tile += step) {
+            const int vkey = tile * kCacheTile + g * 16;
+            const bool held = (uint32_t)ventry < (uint32_t)p.cache.pages && vkey < it.keys;
+            const int exponent = cache_exponent(vs);
+            int now;
+            if (!this->whole(tile * kCacheTile, held, exponent, now)) {
+                any = true;
+                break;
+            }
+            const float c = c0 * ks, scale = vs;
+            kentry = knext, ventry = vnext;
+            // (always loaded, of a tile there is: joining the value with another
+            // would wait for the load here)
+            const int ahead = min(tile + 2 * step, end - 1);
+            knext = entry(ahead, r16 >> 2), vnext = entry(ahead, g);
+            const bool more = tile + step < end;
+            this->step(c, scale, exponent, now, keys, values,
+                       [&] { if (more) load_keys<NT>(p, head, kp, tile + step, kentry, ventry); });
+            if (more) load_values<NT>(p, vp, tile + step, ventry);
+        }
+        if (any)
+            for (; tile < end; tile += step) {
+                const int vkey = tile * kCacheTile + g * 16;
+                const bool held = (uint32_t)ventry < (uint32_t)p.cache.pages && vkey < it.keys;
+                this->step_any(vkey, held, c0 * ks, vs, keys, values, [] {});
+                if (tile + step < end) {
+                    kentry = knext, ventry = vnext;
+                    const int ahead = min(tile + 2 * step, end - 1);
+                    knext = entry(ahead, r16 >> 2), vnext = entry(ahead, g);
+                    load_keys<NT>(p, head, kp, tile + step, kentry, ventry);
+                    load_values<NT>(p, vp, tile + step, ventry);
+                }
+            }
+        this->finish(p, it, begin, end, step, lane);
+    }
+};
+
+// Where the rows of a block end: outputs, or a part of them in the workspace
+// (o [16][D], then m and l [16] each).
+template <int D>
+constexpr int cache_part_floats() { return kCacheRows * (D + 2); }
+
+template <typename T, int D>
+__device__ __forceinline__ void cache_store(const CacheAttnParams &p, const CacheItem &it, int r, int d, cf32x4_t x, float m, float l) {
+    constexpr float kLn2 = 0.693147180559945309f;
+    const int t = it.q0 + (it.row0 + r) / p.group, h = it.head * p.group + (it.row0 + r) % p.group;
+    const float inverse = l == 0.f ? 0.f : 1.f / l;   // nothing seen: 0
+    struct alignas(4 * sizeof(T)) { T v[4]; } y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y.v[e] = (T)(x[e] * inverse);
+    *(decltype(y) *)((T *)p.o + (int64_t)t * p.o_st + (int64_t)h * p.o_sh + d) = y;
+    if (d == 0) {
+        const int64_t at = (int64_t)t * p.kv_heads * p.group + h;
+        p.m[at] = m * kLn2;
+        p.l[at] = l;
+    }
+}
+
+// The waves' results joined.
+template <int D, int NW>
+struct CacheJoin {
+    float o[NW][kCacheRows][D + 4];
+    float m[NW][kCacheRows], l[NW][kCacheRows];
+
+    template <typename T>
+    __device__ __forceinline__ void put(const CacheWave<T, D> &w, int wave, int lane) {
+        const int g = lane >> 4, r16 = lane & 15;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) *(cf32x4_t *)&o[wave][r16][i * 16 + g * 4] = w.o[0][i];
+        if (g == 0) {
+            m[wave][r16] = w.m[0];
+            l[wave][r16] = w.l[0];
+        }
+    }
+    __device__ __forceinline__ cf32x4_t get(int r, int d, float &mx, float &sum) const {
+        mx = m[0][r];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) mx = cache_max(mx, m[w][r]);
         const float ref = mx == -INFINITY ? 0.f : mx;
-        float sum = 0.f;
+        sum = 0.f;
         cf32x4_t x{};
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
-            const float f = __builtin_amdgcn_exp2f(part_m[w][r] - ref);
-            sum += part_l[w][r] * f;
-            x += *(const cf32x4_t *)&part[w][r][d] * f;
+            const float f = __builtin_amdgcn_exp2f(m[w][r] - ref);
+            sum += l[w][r] * f;
+            x += *(const cf32x4_t *)&o[w][r][d] * f;
         }
-        const int t = it.q0 + (it.row0 + r) / p.group, h = it.head * p.group + (it.row0 + r) % p.group;
-        const float inverse = sum == 0.f ? 0.f : 1.f / sum;   // nothing seen: 0
-        struct alignas(4 * sizeof(T)) { T v[4]; } y;
+        return x;
+    }
+};
+
+// A workgroup for each row block, whose NW waves split its tiles.
+template <typename T, int D, int NW>
+__global__ __launch_bounds__(NW * 64, D >= 128 ? 2 : 3) void cache_attn_kernel(CacheAttnParams p) {
+    __shared__ __attribute__((aligned(16))) CacheJoin<D, NW> join;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    CacheItem it;
+    int i = blockIdx.x;
+    if (!cache_find(p, i, lane, it, [&](const CacheItem &r) { return cache_blocks(p, r) * p.kv_heads; })) return;
+    const int blocks = cache_blocks(p, it);
+    it.head = i / blocks;
+    it.row0 = i % blocks * kCacheRows;
+    cache_uniform(it);
+    CacheWave<T, D> w;
+    w.run(p, it, wave, INT32_MAX, NW, lane);
+    join.put(w, wave, lane);
+    __syncthreads();
+    for (int j = tid; j < kCacheRows * D / 4; j += NW * 64) {
+        const int r = j / (D / 4), d = j % (D / 4) * 4;
+        if (it.row0 + r >= cache_rows(p, it)) break;
+        float m, l;
+        const cf32x4_t x = join.get(r, d, m, l);
+        cache_store<T, D>(p, it, r, d, x, m, l);
+    }
+}
+
+// From so many rows on a request is a chunk: where the call has many rows, chunks
+// have a form of their own.
+constexpr int kChunkFrom = 64;
+__device__ __forceinline__ bool cache_is_chunk(const CacheAttnParams &p, const CacheItem &r) { return cache_rows(p, r) >= kChunkFrom; }
+
+// The tiles of all row blocks, one after the other (requests, then heads, then
+// blocks), in equal ranges of a wave each, however the requests' lengths differ:
+// the host need not know them.  A block counts for kBlockCost tiles more than it
+// has, about what its start and end take a wave; they lie before its first.  A
+// block in several ranges leaves a part for each in the workspace, which
+// cache_attn_join_kernel adds up: part 2 w of range w is the one that starts the
+// range, 2 w + 1 one that starts behind it.  `unfinished` tells the join of the
+// block whose first tile is in range w and whose last is not.
+struct CacheUnfinished {
+    int rows;         // of the block, 0: there is none
+    int q0, head, row0;
+    int parts, first; // how many, and the first's number
+    int pad[2];
+};
+constexpr int kBlockCost = 2;
+
+__device__ __forceinline__ int cache_weight(const CacheAttnParams &p, const CacheItem &r) {
+    if (p.chunks && cache_is_chunk(p, r)) return 0;
+    return cache_blocks(p, r) * p.kv_heads * (cache_tiles(r) + kBlockCost);
+}
+
+template <typename T, int D>
+__device__ __forceinline__ void cache_split(const CacheAttnParams &p, int range, int ranges) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, r16 = lane & 15;
+    const auto weight = [&](const CacheItem &r) { return cache_weight(p, r); };
+    const int total = cache_total(p, lane, weight);
+    const int per = (total + ranges - 1) / ranges;
+    const int lo = (int)min((int64_t)range * per, (int64_t)total), hi = min(lo + per, total);
+    CacheUnfinished left{};
+    CacheItem it;
+    int i = lo;                           // the place among the request's
+    if (lo < hi) {
+        cache_find(p, i, lane, it, weight);
+        cache_uniform(it);
+    }
+    CacheWave<T, D> w;
+    for (int at = lo; at < hi;) {
+        const int length = cache_tiles(it) + kBlockCost, blocks = cache_blocks(p, it);
+        const int block = i / length;
+        const int begin = i - block * length, end = min(length, begin + (hi - at));
+        const int from = max(begin - kBlockCost, 0), to = end - kBlockCost;
+        if (to > 0) {
+            it.head = __builtin_amdgcn_readfirstlane(block / blocks);
+            it.row0 = __builtin_amdgcn_readfirstlane(block % blocks * kCacheRows);
+            const int rows = (int)min(cache_rows(p, it) - it.row0, (int64_t)kCacheRows);
+            w.run(p, it, from, to, 1, lane);
+            const int number = 2 * range + (at != lo);
+            const bool all = from == 0 && end == length;
+            if (from == 0 && end < length)
+                left = CacheUnfinished{rows, it.q0, it.head, it.row0, (at - begin + length - 1) / per - range + 1, number, {0, 0}};
+            float *part = p.parts + (int64_t)number * cache_part_floats<D>();
+            if (r16 < rows) {
+                if (all) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y.v[e] = (T)(x[e] * inverse);
-        *(decltype(y) *)((T *)p.o + (int64_t)t * p.o_st + (int64_t)h * p.o_sh + d) = y;
-        if (d == 0) {
-            const int64_t at = (int64_t)t * p.kv_heads * p.group + h;
-            p.m[at] = mx * kLn2;
-            p.l[at] = sum;
+                    for (int j = 0; j < D / 16; ++j) cache_store<T, D>(p, it, r16, j * 16 + g * 4, w.o[0][j], w.m[0], w.l[0]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < D / 16; ++j) *(cf32x4_t *)(part + r16 * D + j * 16 + g * 4) = w.o[0][j];
+                    if (g == 0) {
+                        part[kCacheRows * D + r16] = w.m[0];
+                        part[kCacheRows * (D + 1) + r16] = w.l[0];
+                    }
+                }
+            }
+        }
+        at += end - begin;
+        i += end - begin;
+        if (at < hi && i >= length * blocks * p.kv_heads) {
+            i = 0;
+            do it = cache_request(p, it.b + 1);
+            while (cache_weight(p, it) == 0);
+            cache_uniform(it);
         }
     }
+    if (lane == 0) p.unfinished[range] = left;
+}
+
+constexpr int kSplitWaves = 4;   // of a workgroup: they share nothing
+
+template <typename T, int D>
+__global__ __launch_bounds__(kSplitWaves * 64, D >= 128 ? 2 : 3) void cache_attn_split_kernel(CacheAttnParams p) {
+    cache_split<T, D>(p, blockIdx.x * kSplitWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), p.ranges);
+}
+
+// Workgroup w adds up the parts of the block that range w leaves unfinished, a row
+// to a wave: D / 4 lanes have the columns of a part.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void cache_attn_join_kernel(CacheAttnParams p) {
+    const CacheUnfinished u = p.unfinished[blockIdx.x];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    CacheItem it;
+    it.q0 = u.q0, it.head = u.head, it.row0 = u.row0;
+    constexpr int PF = cache_part_floats<D>();
+    const float *first = p.parts + (int64_t)u.first * PF;
+    const float *rest = p.parts + 2 * (int64_t)blockIdx.x * PF;    // part k > 0 is rest[2 k]
+    const auto part = [&](int k) { return k ? rest + (int64_t)2 * k * PF : first; };
+    constexpr int SL = 64 / (D / 4);                                // parts at a time
+    const int slice = lane / (D / 4), d = lane % (D / 4) * 4;
+    for (int r = wave; r < u.rows; r += 4) {
+        float mx = -INFINITY;
+        for (int k = lane; k < u.parts; k += 64) mx = cache_max(mx, part(k)[kCacheRows * D + r]);
+#pragma unroll
+        for (int x = 1; x < 64; x <<= 1) mx = cache_max(mx, __shfl_xor(mx, x));
+        const float ref = mx == -INFINITY ? 0.f : mx;
+        float sum = 0.f;
+        cf32x4_t x{};
+#pragma unroll 4
+        for (int k = slice; k < u.parts; k += SL) {
+            const float *q = part(k);
+            const float f = __builtin_amdgcn_exp2f(q[kCacheRows * D + r] - ref);
+            sum += q[kCacheRows * (D + 1) + r] * f;
+            x += *(const cf32x4_t *)(q + r * D + d) * f;
+        }
+#pragma unroll
+        for (int y = D / 4; y < 64; y <<= 1) {
+            sum += __shfl_xor(sum, y);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] += __shfl_xor(x[e], y);
+        }
+        if (slice == 0) cache_store<T, D>(p, it, r, d, x, mx, sum);
+    }
+}
+
+// Chunks of prompts: a wave has 32 rows and all their tiles, which its workgroup
+// stages in the LDS, as codes, one tile ahead of the products (16 KB at head_dim
+// 128 for 128 rows: the matrix unit works 4 times as long on a tile as the L2
+// takes to bring it).  In the LDS 16-byte pieces change places within a row, by
+// the row's number, so that the 16 rows that a read takes lie in all banks.
+constexpr int kChunkBlocks = 2, kChunkWaves = 4;
+constexpr int kChunkRows = kCacheRows * kChunkBlocks * kChunkWaves;
+
+template <int D>
+struct CacheStage {
+    static constexpr int KP = D / 16;                  // pieces of a key
+    static constexpr int PIECES = 2 * kCacheTile * KP; // of a tile's keys and values
+    static constexpr int BYTES = PIECES * 16;
+    static constexpr int N = PIECES / (kChunkWaves * 64);   // a thread's
+
+    // place of a key's piece, of a column's
+    static __device__ __forceinline__ int key_swap(int row) {
+        return D == 128 ? (row >> 4 & 3) * 2 + (row >> 1 & 1) : D == 64 ? row >> 4 & 3 : 0;
+    }
+    static __device__ __forceinline__ int value_swap(int d) { return d >> 2 & 3; }
+
+    int32_t entry[N];    // of the pages that the thread's pieces are in
+
+    // First key of the thread's piece n in a tile, the piece's place being
+    // (n * 4 + wave) * 64 + lane: keys first, then values.
+    static __device__ __forceinline__ bool is_key(int n, int wave) { return (n * kChunkWaves + wave) * 64 < PIECES / 2; }
+    static __device__ __forceinline__ int key_of(int n, int wave, int lane) {
+        const int x = (n * kChunkWaves + wave) * 64 + lane;
+        if (is_key(n, wave)) return x / KP;
+        const int y = x - PIECES / 2;
+        return (y % 4 ^ value_swap(y / 4)) * 16;
+    }
+    __device__ __forceinline__ void look_up(const CacheAttnParams &p, const CacheHead &head, int tile, int wave, int lane) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) entry[n] = head.entry(p, tile * kCacheTile + key_of(n, wave, lane));
+    }
+    // the thread's part of a page, and the loads of a tile into `stage`
+    const uint8_t *at[N];
+    __device__ __forceinline__ void place(const CacheAttnParams &p, const CacheHead &head, int wave, int lane) {
+        const int in_page = (1 << p.cache.log2_page) - 1;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int x = (n * kChunkWaves + wave) * 64 + lane, key = key_of(n, wave, lane) & in_page;
+            at[n] = is_key(n, wave) ? head.k + (int64_t)key * p.cache.k_st + (x % KP ^ key_swap(x / KP)) * 16
+                                    : head.v + key + (int64_t)((x - PIECES / 2) / 4) * p.cache.v_sd;
+        }
+    }
+    __device__ __forceinline__ void load(const CacheAttnParams &p, uint8_t *stage, int tile, int wave) const {
+        const int first = tile * kCacheTile & (1 << p.cache.log2_page) - 1;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const bool key = is_key(n, wave);
+            const uint8_t *src = cache_at(at[n], cache_page(p, entry[n]), key ? p.cache.k_sp : p.cache.v_sp) + (uint32_t)(key ? first * p.cache.k_st : first);
+            typedef const __attribute__((address_space(1))) void gvoid;
+            typedef __attribute__((address_space(3))) void lvoid;
+            __builtin_amdgcn_global_load_lds((gvoid *)src, (lvoid *)(stage + (n * kChunkWaves + wave) * 1024), 16, 0, 0);
+        }
+    }
+    static __device__ __forceinline__ CacheCodes key(const uint8_t *stage, int t, int k, int lane) {
+        const int g = lane >> 4, r16 = lane & 15, row = (r16 >> 2) * 16 + 4 * t + (r16 & 3);
+        if constexpr (D >= 64) {
+            const uint4 x = *(const uint4 *)(stage + row * D + ((k / 2 * 4 + g) ^ key_swap(row)) * 16);
+            return k % 2 ? CacheCodes{x.z, x.w} : CacheCodes{x.x, x.y};
+        } else {
+            const uint2 x = *(const uint2 *)(stage + row * D + g * 8);
+            return CacheCodes{x.x, x.y};
+        }
+    }
+    static __device__ __forceinline__ CacheCodes value(const uint8_t *stage, int i, int h, int lane) {
+        const int g = lane >> 4, d = i * 16 + (lane & 15);
+        const uint4 x = *(const uint4 *)(stage + BYTES / 2 + d * 64 + (g ^ value_swap(d)) * 16);
+        return h ? CacheCodes{x.z, x.w} : CacheCodes{x.x, x.y};
+    }
+};
+
+template <typename T, int D>
+__device__ __forceinline__ void cache_chunk(const CacheAttnParams &p, uint8_t *smem, int i) {
+    using Stage = CacheStage<D>;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
+    const auto blocks = [&](const CacheItem &r) {
+        return cache_is_chunk(p, r) ? (int)((cache_rows(p, r) + kChunkRows - 1) / kChunkRows) : 0;
+    };
+    CacheItem it;
+    if (!cache_find(p, i, lane, it, [&](const CacheItem &r) { return blocks(r) * p.kv_heads; })) return;
+    const int n = blocks(it);
+    it.head = i / n;
+    const int row0 = __builtin_amdgcn_readfirstlane(i % n * kChunkRows);
+    it.row0 = row0 + wave * kChunkBlocks * kCacheRows;
+    cache_uniform(it);
+    const int64_t rows = cache_rows(p, it);
+    const int tiles = (cache_limit(p, it, (int)(min((int64_t)row0 + kChunkRows, rows) - 1) / p.group) + kCacheTile - 1) / kCacheTile;
+
+    CacheRows<T, D, kChunkBlocks> w;
+    w.load(p, it, lane);
+    if (tiles > 0) {
+        const CacheHead head(p, it);
+        const auto entry = [&](int tile) { return head.entry(p, tile * kCacheTile + g * 16); };
+        Stage stage;
+        stage.place(p, head, wave, lane);
+        stage.look_up(p, head, 0, wave, lane);
+        int now = entry(0), next = entry(min(1, tiles - 1));
+        stage.load(p, smem, 0, wave);
+        uint32_t page = cache_page(p, now);
+        float next_ks = *(const float *)cache_at(head.ks, page, p.cache.ks_sp), next_vs = *(const float *)cache_at(head.vs, page, p.cache.vs_sp);
+        stage.look_up(p, head, min(1, tiles - 1), wave, lane);
+        const float c0 = p.scale * 1.44269504088896341f;
+        for (int tile = 0; tile < tiles; ++tile) {
+            // this tile's loads have ended, and all waves have done with the other stage
+            __builtin_amdgcn_s_waitcnt(0);
+            __syncthreads();
+            const float ks = next_ks, vs = next_vs;
+            const int key0 = tile * kCacheTile, vkey = key0 + g * 16;
+            const bool held = (uint32_t)now < (uint32_t)p.cache.pages && vkey < it.keys;
+            now = next;
+            if (tile + 1 < tiles) stage.load(p, smem + (tile + 1 & 1) * Stage::BYTES, tile + 1, wave);
+            // (always loaded, of a tile there is: joining the values with others would
+            // wait for the loads here)
+            page = cache_page(p, now);
+            next_ks = *(const float *)cache_at(head.ks, page, p.cache.ks_sp);
+            next_vs = *(const float *)cache_at(head.vs, page, p.cache.vs_sp);
+            const int ahead = min(tile + 2, tiles - 1);
+            stage.look_up(p, head, ahead, wave, lane);
+            next = entry(ahead);
+            if (key0 >= w.last_limit) continue;
+            const uint8_t *codes = smem + (tile & 1) * Stage::BYTES;
+            const auto keys = [&](int t, int k) { return Stage::key(codes, t, k, lane); };
+            const auto values = [&](int i, int h) { return Stage::value(codes, i, h, lane); };
+            const int exponent = cache_exponent(vs);
+            int largest;
+            if (w.whole(key0, held, exponent, largest))
+                w.step(c0 * ks, vs, exponent, largest, keys, values, [] {});
+            else
+                w.step_any(vkey, held, c0 * ks, vs, keys, values, [] {});
+        }
+    }
+    if (it.row0 >= rows) return;
+    w.finish(p, it, 0, (w.last_limit + kCacheTile - 1) / kCacheTile, 1, lane);
+#pragma unroll
+    for (int b = 0; b < kChunkBlocks; ++b) {
+        const int r = b * kCacheRows + (lane & 15);
+        if (it.row0 + r < rows) {
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) cache_store<T, D>(p, it, r, i * 16 + g * 4, w.o[b][i], w.m[b], w.l[b]);
+        }
+    }
+}
+
+// Both forms in one launch: first the ranges of the requests with few rows, then
+// the chunks.
+template <typename T, int D>
+__global__ __launch_bounds__(kChunkWaves * 64, 2) void cache_attn_mixed_kernel(CacheAttnParams p) {
+    static_assert(kSplitWaves == kChunkWaves, "one workgroup shape");
+    __shared__ __attribute__((aligned(16))) uint8_t smem[2 * CacheStage<D>::BYTES];
+    const int split = p.ranges / kSplitWaves;
+    if ((int)blockIdx.x < split)
+        cache_split<T, D>(p, blockIdx.x * kSplitWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), p.ranges);
+    else
+        cache_chunk<T, D>(p, smem, blockIdx.x - split);
 }
 
 }  // namespace pmkl_amd

@@ -118,14 +118,16 @@ int fill_cache(const pmkl_kv_cache &c, bool written, CacheParams *p) {
     PMKL_TRY(check_strides("v_cache", {{vs[0], P}, {vs[1], H}, {vs[2], D}}, ps, 16, written));
     PMKL_TRY(check_strides("k_scale", {{kss[0], P}, {kss[1], H}}, 1, 1, written));
     PMKL_TRY(check_strides("v_scale", {{vss[0], P}, {vss[1], H}}, 1, 1, written));
+    PMKL_REQUIRE(ks[0] <= INT32_MAX && vs[0] <= INT32_MAX && kss[0] <= INT32_MAX / 4 && vss[0] <= INT32_MAX / 4,
+                 PMKL_EINVAL, "pages lie more than 2 GiB apart");
     p->k = (uint8_t *)c.k;
     p->v = (uint8_t *)c.v;
     p->k_scale = c.k_scale;
     p->v_scale = c.v_scale;
-    p->k_sp = ks[0], p->k_sh = ks[1], p->k_st = (int32_t)ks[2];
-    p->v_sp = vs[0], p->v_sh = vs[1], p->v_sd = (int32_t)vs[2];
-    p->ks_sp = kss[0], p->ks_sh = kss[1];
-    p->vs_sp = vss[0], p->vs_sh = vss[1];
+    p->k_sp = (uint32_t)ks[0], p->k_sh = ks[1], p->k_st = (int32_t)ks[2];
+    p->v_sp = (uint32_t)vs[0], p->v_sh = vs[1], p->v_sd = (int32_t)vs[2];
+    p->ks_sp = (uint32_t)(kss[0] * 4), p->ks_sh = kss[1];
+    p->vs_sp = (uint32_t)(vss[0] * 4), p->vs_sh = vss[1];
     p->pages = (int32_t)P;
     p->log2_page = log2_of(ps);
     return PMKL_OK;
@@ -259,20 +261,32 @@ int run_append(const pmkl_cache_append_args *a, void *stream) {
 
 typedef void (*cache_attn_fn)(CacheAttnParams);
 constexpr int kAttnWaves = 4;
+constexpr int64_t kChunkRows = pmkl_amd::kChunkRows;
+constexpr int64_t kWholeKeys = 1024;
 
+struct AttnKernels {
+    cache_attn_fn whole, split, mixed, join;
+};
+
+template <typename T, int D>
+AttnKernels attn_kernels() {
+    return {pmkl_amd::cache_attn_kernel<T, D, kAttnWaves>, pmkl_amd::cache_attn_split_kernel<T, D>,
+            pmkl_amd::cache_attn_mixed_kernel<T, D>, pmkl_amd::cache_attn_join_kernel<T, D>};
+}
 template <typename T>
-cache_attn_fn pick_attn(int64_t D) {
+AttnKernels pick_attn(int64_t D) {
     switch (D) {
-        case 32: return pmkl_amd::cache_attn_kernel<T, 32, kAttnWaves>;
-        case 64: return pmkl_amd::cache_attn_kernel<T, 64, kAttnWaves>;
-        default: return pmkl_amd::cache_attn_kernel<T, 128, kAttnWaves>;
+        case 32: return attn_kernels<T, 32>();
+        case 64: return attn_kernels<T, 64>();
+        default: return attn_kernels<T, 128>();
     }
 }
 
 struct AttnPlan {
-    cache_attn_fn fn;
-    int64_t grid;
-    uint64_t workspace;
+    AttnKernels fn;
+    bool split, mixed;   // (mixed: split too)
+    int64_t grid, ranges;
+    uint64_t parts, workspace;   // bytes: of the split form's parts, in all
     bool empty;
 };
 
@@ -302,8 +316,24 @@ int plan_attn(const pmkl_cache_attn_args *a, AttnPlan *pl) {
     const int64_t D = a->cache.head_dim, G = a->heads / a->cache.kv_heads;
     pl->fn = a->dtype == PMKL_DTYPE_F32 ? pick_attn<float>(D)
              : a->dtype == PMKL_DTYPE_F16 ? pick_attn<_Float16>(D) : pick_attn<__bf16>(D);
-    // every request's last tile may be partly filled; a request without tokens has none
-    pl->grid = (a->tokens * G / 16 + std::min(a->batch, a->tokens)) * a->cache.kv_heads;
+    // every request's last block may be partly filled; a request without tokens has none
+    pl->grid = (a->tokens * G / pmkl_amd::kCacheRows + std::min(a->batch, a->tokens)) * a->cache.kv_heads;
+    // the split form counts tiles of all row blocks in 32 bits
+    const int64_t tiles = (a->table_width * a->cache.page_size + pmkl_amd::kCacheTile - 1) / pmkl_amd::kCacheTile +
+                          pmkl_amd::kBlockCost;
+    pl->split = a->table_width * a->cache.page_size > kWholeKeys && pl->grid <= INT32_MAX / tiles;
+    if (pl->split) {
+        // as many waves as the chip's 1,024 SIMDs hold of the kernel
+        const int64_t heads = a->cache.kv_heads, rows = a->tokens * G;
+        pl->mixed = rows * heads >= kChunkRows * 256;
+        pl->ranges = 1024 * (D >= 128 || pl->mixed ? 2 : 3);
+        pl->grid = pl->ranges / pmkl_amd::kSplitWaves;
+        pl->parts = (uint64_t)2 * pl->ranges * pmkl_amd::kCacheRows * (D + 2) * sizeof(float);
+        pl->workspace = pl->parts + pl->ranges * sizeof(pmkl_amd::CacheUnfinished);
+        // enough rows for a workgroup of 128 on every CU: chunks in their own form
+        if (pl->mixed)
+            pl->grid += (rows / kChunkRows + std::min(std::min(a->batch, a->tokens), rows / pmkl_amd::kChunkFrom)) * heads;
+    }
     PMKL_REQUIRE(pl->grid * kAttnWaves * 64 < (int64_t(1) << 32), PMKL_EINVAL, "grid too large (%lld workgroups)",
                  (long long)pl->grid);
     return PMKL_OK;
@@ -331,6 +361,13 @@ int run_attn(const pmkl_cache_attn_args *a, void *stream) {
     p.table_stride = a->table_stride ? a->table_stride : a->table_width;
     PMKL_REQUIRE(p.table_stride >= 0 && p.table_stride <= (int64_t(1) << 40), PMKL_EINVAL,
                  "table_stride %lld is not in 0 .. 2^40", (long long)p.table_stride);
+    if (pl.split) {
+        PMKL_TRY(check_pointer("workspace", a->workspace, 16));
+        PMKL_REQUIRE(a->workspace_bytes >= pl.workspace, PMKL_EINVAL, "workspace of %llu bytes is too small (needs %llu)",
+                     (unsigned long long)a->workspace_bytes, (unsigned long long)pl.workspace);
+    }
+    p.parts = (float *)a->workspace;
+    p.unfinished = (pmkl_amd::CacheUnfinished *)((char *)a->workspace + pl.parts);
     p.q = a->q;
     p.o = a->o;
     p.m = a->m;
@@ -345,8 +382,14 @@ int run_attn(const pmkl_cache_attn_args *a, void *stream) {
     p.group = (int32_t)(H / a->cache.kv_heads);
     p.is_causal = a->is_causal ? 1 : 0;
     p.scale = a->scale > 0.f ? a->scale : 1.0f / std::sqrt((float)D);
-    hipLaunchKernelGGL(pl.fn, dim3((unsigned)pl.grid), dim3(kAttnWaves * 64), 0, (hipStream_t)stream, p);
-    return launched("cache_attn");
+    p.ranges = (int32_t)pl.ranges;
+    p.chunks = pl.mixed ? 1 : 0;
+    hipLaunchKernelGGL(pl.mixed ? pl.fn.mixed : pl.split ? pl.fn.split : pl.fn.whole, dim3((unsigned)pl.grid), dim3(kAttnWaves * 64), 0,
+                       (hipStream_t)stream, p);
+    PMKL_TRY(launched("cache_attn"));
+    if (!pl.split) return PMKL_OK;
+    hipLaunchKernelGGL(pl.fn.join, dim3((unsigned)pl.ranges), dim3(256), 0, (hipStream_t)stream, p);
+    return launched("cache_attn_join");
 }
 
 }  // namespace
@@ -381,8 +424,11 @@ const char *pmkl_cache_attn_kernel_name(const pmkl_cache_attn_args *a) {
     if (plan_attn(a, &pl) != PMKL_OK) return nullptr;
     if (pl.empty) return "none";
     const char *dt = a->dtype == PMKL_DTYPE_BF16 ? "bf16" : a->dtype == PMKL_DTYPE_F16 ? "fp16" : "fp32";
-    snprintf(name, sizeof(name), "cache_attn_kernel<%s, %lld, %d> grid %lld x %d", dt, (long long)a->cache.head_dim,
-             kAttnWaves, (long long)pl.grid, kAttnWaves * 64);
+    const int n = snprintf(name, sizeof(name), "cache_attn_%skernel<%s, %lld> grid %lld x %d", pl.mixed ? "mixed_" : pl.split ? "split_" : "",
+                           dt, (long long)a->cache.head_dim, (long long)pl.grid, kAttnWaves * 64);
+    if (pl.split)
+        snprintf(name + n, sizeof(name) - n, ", cache_attn_join_kernel<%s, %lld> grid %lld x 256", dt,
+                 (long long)a->cache.head_dim, (long long)pl.ranges);
     return name;
 }
 

@@ -8,17 +8,16 @@
 
 namespace pmkl_amd {
 
-// pmkl_kv_cache with its strides filled in (bytes of the codes, elements of
-// the scales).
+// pmkl_kv_cache with its strides filled in, in bytes but for the scales' heads.
 struct CacheParams {
     uint8_t *k;
     uint8_t *v;
     float *k_scale;
     float *v_scale;
-    int64_t k_sp, k_sh;     // page, head
-    int64_t v_sp, v_sh;
-    int64_t ks_sp, ks_sh;
-    int64_t vs_sp, vs_sh;
+    int64_t k_sh, v_sh;     // head
+    int64_t ks_sh, vs_sh;   // (elements)
+    uint32_t k_sp, v_sp;    // page, below 2^31
+    uint32_t ks_sp, vs_sp;
     int32_t k_st, v_sd;     // token of k, column of v
     int32_t pages;
     int32_t log2_page;
@@ -48,7 +47,17 @@ __device__ __forceinline__ float wave_max(float x) {
     return across_rows(x, op);
 }
 
-// Inclusive sums over the wave's lanes.
+// Inclusive sums over the wave's lanes: within rows of 16, then the rows' sums
+// to the rows behind.
+__device__ __forceinline__ int wave_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);   // row_shr 1, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);   // row_bcast 15, to rows 1 and 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);   // row_bcast 31, to rows 2 and 3
+    return x;
+}
 __device__ __forceinline__ int64_t wave_scan(int64_t x, int lane) {
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {

@@ -251,8 +251,8 @@ __global__ __launch_bounds__(kCacheThreads) void cache_append_kernel(AppendParam
             a = finite_max(*(const CacheVec<T, E> *)(x + i * st + lane % LPR * E), a);
         a = wave_max(a);
 
-        float *scale = which ? p.cache.v_scale + page * p.cache.vs_sp + head * p.cache.vs_sh
-                             : p.cache.k_scale + page * p.cache.ks_sp + head * p.cache.ks_sh;
+        float *scale = which ? p.cache.v_scale + page * (p.cache.vs_sp / 4) + head * p.cache.vs_sh
+                             : p.cache.k_scale + page * (p.cache.ks_sp / 4) + head * p.cache.ks_sh;
         const float was = *scale, need = cache_scale_for(a);
         const bool kept = o > 0 && was > 0.f && was < INFINITY;
         const float now = kept ? fmaxf(was, need) : need;

@@ -93,23 +93,26 @@ def append(k, v, slot, k_codes, v_codes, k_scale, v_scale):
     return caches[0][1], caches[1][1].swapaxes(2, 3), caches[0][2], caches[1][2]
 
 
-def attend(q, k_codes, v_codes, k_scale, v_scale, table, seq_lens, query_start, causal, scale, dtype, term_error=None):
+def attend(q, k_codes, v_codes, k_scale, v_scale, table, seq_lens, query_start, causal, scale, dtype):
     """out, m, l in float64 and the bounds of their errors, all [N, heads(, D)]; rows of no request are NaN with a bound of
     -1.
 
     Bounds.  A score is a sum of D products in fp32, of terms that hold q and k exactly, times three fp32 factors: off by at
     most ds = (D + 8) 2^-24 scale sum_d |q_d k_d| (its largest over the row's keys).  A weight exp(s - m) is off by 2 ds
     (s and m) and by 2^-21 (the exponent's rounding for |s - m| < 8, larger differences weigh less; exp2; the factor of the
-    values' scale), and by what is left of its bf16 terms (two: 2^-17, three: 2^-24).  Sums over L keys are made of at
+    values' scale), and by the rounding of its f16 terms.  A term has 11 significant bits, so it is off by at most half of
+    its last one, 2^-11 of itself: under bf16 queries, with one term, each w_j v_j is off by 2^-11 |w_j v_j|, and the
+    ratio by 2^-11 sum w |v| / sum w (an eighth of a bf16 output's own half step, 2^-8); with two terms by 2^-22.  Sums over L keys are made of at
     most L / 32 + 64 additions to one accumulator, each off by 2^-24 of the sum of magnitudes.  The output is a ratio of two
-    such sums, rounded once."""
+    such sums, rounded once: by half a step of its type, which for numbers below fp16's least normal one, 2^-14, is
+    half of its least step of 2^-24 (bf16's and fp32's are below 1e-30, which stands for them)."""
     n_tokens, heads, D = q.shape
     page_size, kv_heads = k_codes.shape[2], k_codes.shape[1]
     group = heads // kv_heads
     out = np.full(q.shape, np.nan)
     m, l = np.full(q.shape[:2], np.nan), np.full(q.shape[:2], np.nan)
     out_bound, m_bound, l_bound = np.full(q.shape, -1.0), np.full(m.shape, -1.0), np.full(m.shape, -1.0)
-    terms = term_error if term_error is not None else 2.0 ** -24 if dtype == "fp32" else 2.0 ** -17
+    terms = 2.0 ** -11 if dtype == "bf16" else 2.0 ** -22
     for b in range(len(seq_lens)):
         lo, hi = int(query_start[b]), int(query_start[b + 1])
         keys = min(int(seq_lens[b]), table.shape[1] * page_size)
@@ -117,27 +120,32 @@ def attend(q, k_codes, v_codes, k_scale, v_scale, table, seq_lens, query_start, 
         page = table[b, at // page_size]
         held = (page >= 0) & (page < k_codes.shape[0])
         page = np.where(held, page, 0)
+        if lo == hi:
+            continue
+        position = int(seq_lens[b]) - (hi - lo) + np.arange(hi - lo)
+        seen = held & ((at <= position[:, None]) if causal else np.ones((hi - lo, keys), bool))
+        some = seen.any(1)
         for h in range(heads):
             g = h // group
-            kk = E4M3[k_codes[page, g, at % page_size]] * k_scale[page, g][:, None]
-            vv = E4M3[v_codes[page, g, :, at % page_size]] * v_scale[page, g][:, None]
-            for t in range(lo, hi):
-                position = int(seq_lens[b]) - (hi - lo) + (t - lo)
-                seen = held & ((at <= position) if causal else np.ones(keys, bool))
-                if not seen.any():
-                    out[t, h], m[t, h], l[t, h] = 0, -np.inf, 0
-                    out_bound[t, h] = m_bound[t, h] = l_bound[t, h] = 0
-                    continue
-                s = scale * (kk[seen] @ q[t, h])
-                m[t, h] = s.max()
-                p = np.exp(s - m[t, h])
-                l[t, h] = p.sum()
-                out[t, h] = p @ vv[seen] / l[t, h]
-                ds = (D + 8) * 2.0 ** -24 * scale * (np.abs(kk[seen]) @ np.abs(q[t, h])).max()
-                sums = (seen.sum() / 32 + 64) * 2.0 ** -24
-                m_bound[t, h] = ds + 2.0 ** -23 * abs(m[t, h])
-                l_bound[t, h] = l[t, h] * (2 * ds + 2.0 ** -21 + sums)
-                mean = p @ np.abs(vv[seen]) / l[t, h]
-                out_bound[t, h] = HALF_STEP[dtype] * np.abs(out[t, h]) * 1.01 + \
-                    mean * (2 * (2 * ds + 2.0 ** -21 + sums) + terms) + 1e-30
+            kk = E4M3[k_codes[page, g, at % page_size]] * k_scale[page, g][:, None].astype(np.float64)
+            vv = E4M3[v_codes[page, g, :, at % page_size]] * v_scale[page, g][:, None].astype(np.float64)
+            rows = slice(lo, hi)
+            s = np.where(seen, scale * (q[rows, h] @ kk.T), -np.inf)
+            mx = s.max(1, initial=-np.inf)
+            p = np.exp(s - np.where(some, mx, 0.0)[:, None])
+            total = p.sum(1)
+            # a NaN value reaches the rows that see its token, hidden ones (p = 0) none
+            bad = (seen.astype(float) @ np.isnan(vv)) > 0
+            vv = np.nan_to_num(vv, nan=0.0)
+            safe = np.where(some, total, 1.0)[:, None]
+            out[rows, h] = np.where(bad, np.nan, p @ vv / safe)
+            m[rows, h], l[rows, h] = mx, total
+            size = scale * (np.abs(q[rows, h]) @ np.abs(kk).T)
+            ds = (D + 8) * 2.0 ** -24 * np.where(seen, size, 0.0).max(1, initial=0.0)
+            sums = (seen.sum(1) / 32 + 64) * 2.0 ** -24
+            m_bound[rows, h] = np.where(some, ds + 2.0 ** -23 * np.abs(np.where(some, mx, 0.0)), 0.0)
+            l_bound[rows, h] = total * (2 * ds + 2.0 ** -21 + sums)
+            mean = p @ np.abs(vv) / safe
+            out_bound[rows, h] = HALF_STEP[dtype] * np.abs(out[rows, h]) * 1.01 + \
+                mean * (2 * (2 * ds + 2.0 ** -21 + sums) + terms)[:, None] + some[:, None] * (2.0 ** -25 if dtype == "fp16" else 1e-30)
     return (out, m, l), (out_bound, m_bound, l_bound)

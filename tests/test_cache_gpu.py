@@ -160,6 +160,50 @@ def test_long_contexts(device, dtype):
     _attend(cache, _q(sum(new), 8, 64, dtype, seed=3), new, label=dtype)
 
 
+def _form(cache, q):
+    """The kernels that the library chooses for these sizes."""
+    from pmkl_amd import capi
+
+    pages, kv_heads, page, dim = cache.k.shape
+    a = capi.make_cache_attn_args(capi.make_kv_cache(0, 0, 0, 0, pages=pages, kv_heads=kv_heads, page_size=page, head_dim=dim),
+                                  dtype={2: capi.PMKL_DTYPE_BF16, 4: capi.PMKL_DTYPE_F32}[q.element_size()],
+                                  tokens=q.shape[0], heads=q.shape[1], batch=cache.table.shape[0],
+                                  table_width=cache.table.shape[1])
+    return capi.cache_attn_kernel_name(a).split("_kernel")[0]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("dim,page,kv_heads,group,causal", [
+    (128, 16, 4, 8, True), (64, 128, 8, 4, True), (32, 32, 16, 3, True), (128, 64, 2, 16, False)])
+def test_chunks(device, dtype, dim, page, kv_heads, group, causal):
+    """Chunks of prompts beside single tokens, in the form for calls of many rows: chunks that fill their row blocks or
+    not, with and without cached tokens before them, of the whole request and longer than what is cached; a hidden page
+    in one, a NaN value in another, scales far apart in a third."""
+    _say(f"chunks {dtype} D{dim} page {page} heads {kv_heads}x{group} causal={causal}")
+    new = [520, 1, 129, 300, 0, 64, 1, 90]
+    lengths = [1100, 700, 129, 640, 50, 65, 1, 30]
+    cache = Cache(lengths, kv_heads, page, dim, seed=dim + page, interleaved=page == 64)
+    cache.table[0, 300 // page] = -1
+    page3, off = cache.table[3, 500 // page], 500 % page
+    cache.v[page3, 0, 7, off] = 0x7f
+    cache.v_scale[cache.table[2, 0]] *= 2.0 ** 30 if dtype != "fp16" else 2.0 ** 4
+    cache.v_scale[cache.table[5, -(-65 // page) - 1]] *= 2.0 ** -30
+    cache.refresh()
+    q = _q(sum(new) + 10, kv_heads * group, dim, dtype, seed=dim)
+    assert _form(cache, q) == "cache_attn_mixed"
+    out, m, l = _attend(cache, q, new, causal=causal, label=f"{dtype} {dim}")
+    if causal:
+        # request 3: rows 650 .. 949 stand at 340 .. 639
+        assert not out[650:810].isnan().any() and out[810:950, :group, 7].isnan().all()
+
+
+def test_forms(device):
+    """The sizes of these tests reach every form."""
+    for lengths, tokens, heads, form in (([1000], 1, 4, "cache_attn"), ([1100], 1, 4, "cache_attn_split"),
+                                         ([1100], 2000, 32, "cache_attn_mixed")):
+        assert _form(Cache(lengths, 2, 16, 64, seed=1, width_more=0), _q(tokens, heads, 64, "bf16", 1)) == form
+
+
 def test_one_long_request(device):
     lengths = [20000]
     cache = Cache(lengths, 1, 32, 128, seed=10)
