@@ -21,13 +21,13 @@
 //     of this one's, its values after P V, its table entries a tile earlier: 16
 //     KB (head_dim 128) of a wave are under way at any time.
 // Types.  Keys meet bf16 and fp32 queries in bf16 (the latter as three terms, 24
-// bits), f16 queries in f16.  P V is in f16: a weight times its page's scale is
-// (p m 2^14) (v 2^(e - E)) 2^(E - 14), with the scale m 2^e and the tile's largest
-// e as E.  The first factor is one f16 term under bf16 queries (error 2^-12 of a
-// weight, beside the output's 2^-9), two under the others (2^-22); the second is
-// exact, and free in the conversion, while e >= E - 14 (a tile whose scales lie
-// further apart takes another round for the larger ones); the third goes into the
-// factor that rescales the output anyway.
+// bits), f16 queries in f16.  P V is in f16: a weight times its page's scale, s, is
+// held as p s 2^(14 - E), with the exponent of the tile's largest scale as E, and
+// 2^(E - 14) goes into the factor that rescales the output anyway.  That is one f16
+// term under bf16 queries (error 2^-12 of a weight, beside the output's 2^-9) and
+// two under the others (2^-22), in full while the scales of a tile lie within 2^8
+// and p is above 2^-20 (below, 2^-31 is lost); a tile whose scales lie further apart
+// takes another round for the larger ones.
 #pragma once
 
 #include "cache_common.hpp"
@@ -68,7 +68,8 @@ struct CacheAttnParams {
 
 constexpr int kCacheTile = 64;    // keys
 constexpr int kCacheRows = 16;    // query rows of a block
-constexpr int kPBits = 14;        // weights are held as p * 2^14
+constexpr int kPBits = 14;        // weights are held as p s 2^(14 - E)
+constexpr int kSpread = 8;        // scales of a product lie within 2^8
 
 // Queries of a type: the 16-bit type of the score product, how many terms a
 // query has there, and a weight in f16.
@@ -93,20 +94,20 @@ __device__ __forceinline__ cf32x4_t cache_mfma(cf16x8_t a, cf16x8_t b, cf32x4_t 
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// eight codes as an operand, times a power of two
+// eight codes as an operand
 template <typename F>
-__device__ __forceinline__ F cache_frag(uint32_t lo, uint32_t hi, float scale = 1.f) {
+__device__ __forceinline__ F cache_frag(uint32_t lo, uint32_t hi) {
     if constexpr (__is_same(F, cbf16x8_t)) {
-        const cbf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false);
-        const cbf16x2_t b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
-        const cbf16x2_t c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false);
-        const cbf16x2_t d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
+        const cbf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, false);
+        const cbf16x2_t b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, true);
+        const cbf16x2_t c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, false);
+        const cbf16x2_t d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, true);
         return F{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
     } else {
-        const cf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, scale, false);
-        const cf16x2_t b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, scale, true);
-        const cf16x2_t c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, scale, false);
-        const cf16x2_t d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, scale, true);
+        const cf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, false);
+        const cf16x2_t b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, true);
+        const cf16x2_t c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, false);
+        const cf16x2_t d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, true);
         return F{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
     }
 }
@@ -129,6 +130,18 @@ __device__ __forceinline__ float cache_max(float a, float b) { return __builtin_
 
 // Whether a byte of x is the code of NaN (0x7f, 0xff): the high bit of each.
 __device__ __forceinline__ uint32_t cache_nan_bytes(uint32_t x) { return ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
+// 16 codes of a column without those past the first `n`, and 0 for NaN (nans collects where).
+__device__ __forceinline__ void cache_clear(uint32_t (&x)[4], int n, uint32_t &nans) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int some = min(max(n - 4 * j, 0), 4);
+        x[j] &= some ? 0xffffffffu >> (32 - 8 * some) : 0u;
+        const uint32_t bad = cache_nan_bytes(x[j]);
+        nans |= bad;
+        x[j] &= ~(bad | (bad - (bad >> 7)));
+    }
+}
 
 // Over the four 16-lane rows, of an integer that is the same in all lanes of a row.
 template <typename Op>
@@ -238,9 +251,6 @@ __device__ __forceinline__ uint32_t cache_page(const CacheAttnParams &p, int ent
 template <typename T>
 __device__ __forceinline__ const T *cache_at(const T *base, uint32_t page, uint32_t stride) { return base + (uint64_t)page * stride; }
 
-// Two dwords: eight codes.
-struct CacheCodes { uint32_t lo, hi; };
-
 // A wave's rows: QB blocks of 16, of one request and key head, a column of the
 // results each.
 template <typename T, int D, int QB>
@@ -257,7 +267,7 @@ struct CacheRows {
     int limit[QB];          // keys that the lane's row sees
     int first_limit, last_limit;   // that the wave's first and last row see
     int unit, peak;
-    uint32_t nans;          // what masked tiles had to clear
+    uint32_t nans;          // what values() had to clear in tiles for step_any()
 
     // rows it.row0 + 16 b + column, as operands
     __device__ __forceinline__ void load(const CacheAttnParams &p, const CacheItem &it, int lane) {
@@ -310,8 +320,7 @@ struct CacheRows {
             for (int b = 0; b < QB; ++b) s[b][t] = cf32x4_t{};
 #pragma unroll
             for (int k = 0; k < NK; ++k) {
-                const CacheCodes x = keys(t, k);
-                const frag a = cache_frag<frag>(x.lo, x.hi);
+                const frag a = keys(t, k);
 #pragma unroll
                 for (int i = QT - 1; i >= 0; --i)    // the smallest first
 #pragma unroll
@@ -342,120 +351,97 @@ struct CacheRows {
         }
     }
 
+    // o = o alpha + P V, P being s times the lane's weight (where seen[b] > e)
+    template <bool MASKED, typename V>
+    __device__ __forceinline__ void add(const cf32x4_t (&s)[QB][4], const float (&alpha)[QB], float weight, int now, const int (&seen)[QB], V values) {
+        float rescale[QB];
+        bool still = true;
+#pragma unroll
+        for (int b = 0; b < QB; ++b) {
+            rescale[b] = __builtin_amdgcn_ldexpf(alpha[b], unit - now);
+            still = still && rescale[b] == 1.f;
+        }
+        unit = now;
+        peak = max(peak, now);
+        // after the first tiles the largest score seldom changes
+        if (__builtin_amdgcn_ballot_w64(!still) != 0)
+#pragma unroll
+            for (int b = 0; b < QB; ++b)
+#pragma unroll
+                for (int i = 0; i < NB; ++i) o[b][i] *= rescale[b];
+        // eight of the lane's keys, then the others
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            cf16x8_t ph[QB][PT];
+#pragma unroll
+            for (int b = 0; b < QB; ++b)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    float x = s[b][h * 2 + e / 4][e % 4] * weight;
+                    if (MASKED && h * 8 + e >= seen[b]) x = 0.f;   // (of a page that the row does not see the weight may be anything)
+                    _Float16 terms[PT];
+                    cache_terms<PT>(x, terms);
+#pragma unroll
+                    for (int i = 0; i < PT; ++i) ph[b][i][e] = terms[i];
+                }
+#pragma unroll
+            for (int i = 0; i < NB; ++i) {
+                const cf16x8_t a = values(i, h);
+#pragma unroll
+                for (int j = PT - 1; j >= 0; --j)
+#pragma unroll
+                    for (int b = 0; b < QB; ++b) o[b][i] = cache_mfma(a, ph[b][j], o[b][i]);
+            }
+        }
+    }
+
     // A tile that every row sees whole, of pages of the cache whose scales lie
-    // within 2^14 (their exponents' largest is `now`): nearly all tiles.
-    // keys(t, k) and values(i, h) give the operands' codes; taken() is called
-    // when the keys have been taken.
+    // within 2^8 (their exponents' largest is `now`): nearly all tiles.  keys(t, k)
+    // and values(i, h) give the operands; taken() is called when the keys have
+    // been taken.
     template <typename K, typename V, typename F>
-    __device__ __forceinline__ void step(float c, float vs, int exponent, int now, K keys, V values, F taken) {
+    __device__ __forceinline__ void step(float c, float vs, int now, K keys, V values, F taken) {
         cf32x4_t s[QB][4];
         float alpha[QB];
         scores(s, keys);
         taken();
         weigh(s, c, alpha);
-        const float weight = __builtin_amdgcn_ldexpf(vs, kPBits - exponent), vscale = __builtin_amdgcn_ldexpf(1.f, exponent - now);
-        cf16x8_t ph[QB][PT][2];
-#pragma unroll
-        for (int b = 0; b < QB; ++b) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                _Float16 terms[PT];
-                cache_terms<PT>(s[b][e / 4][e % 4] * weight, terms);
-#pragma unroll
-                for (int i = 0; i < PT; ++i) ph[b][i][e / 8][e % 8] = terms[i];
-            }
-            const float rescale = __builtin_amdgcn_ldexpf(alpha[b], unit - now);
-#pragma unroll
-            for (int i = 0; i < NB; ++i) o[b][i] *= rescale;
-        }
-        unit = now;
-        peak = max(peak, now);
-#pragma unroll
-        for (int i = 0; i < NB; ++i)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const CacheCodes x = values(i, h);
-                const cf16x8_t a = cache_frag<cf16x8_t>(x.lo, x.hi, vscale);
-#pragma unroll
-                for (int j = PT - 1; j >= 0; --j)
-#pragma unroll
-                    for (int b = 0; b < QB; ++b) o[b][i] = cache_mfma(a, ph[b][j][h], o[b][i]);
-            }
+        add<false>(s, alpha, __builtin_amdgcn_ldexpf(vs, kPBits - now), now, limit, values);
     }
 
     // Any other tile; its lane has keys vkey .. vkey + 15, `held` if their page is
-    // one of the cache's.
+    // one of the cache's.  values() gives 0 for NaN, and for what no row sees;
+    // anew() keeps what they give from being held over the rounds (64 registers).
     template <typename K, typename V, typename F>
-    __device__ __forceinline__ void step_any(int vkey, bool held, float c, float vs, K keys, V values, F taken) {
+    __device__ __forceinline__ void step_any(int vkey, bool held, float c, float vs, K keys, V values, F anew) {
         cf32x4_t s[QB][4];
         float alpha[QB];
+        int seen[QB];                                      // of the lane's 16 keys, those below are visible
         scores(s, keys);
-        taken();
 #pragma unroll
         for (int b = 0; b < QB; ++b) {
-            const int seen = held ? limit[b] - vkey : 0;   // of the lane's 16 keys, those below are visible
+            seen[b] = held ? limit[b] - vkey : 0;
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 const float x = s[b][e / 4][e % 4] * c;
-                s[b][e / 4][e % 4] = e < seen ? x : -INFINITY;
+                s[b][e / 4][e % 4] = e < seen[b] ? x : -INFINITY;
             }
         }
         weigh(s, 1.f, alpha);
-        // Hidden values count for nothing, also where they are NaN: what no row of
-        // the wave sees is cleared, and a NaN that some see is 0 here and put into
-        // these rows' outputs in the end.
-        uint32_t clear[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int n = held ? min(max(last_limit - vkey - 4 * j, 0), 4) : 0;
-            clear[j] = n ? 0xffffffffu >> (32 - 8 * n) : 0u;
-        }
-        // Pages within 2^14 of the least scale take part together, then the others.
+        // Pages within 2^8 of the least scale take part together, then the others.
         const float scale = held ? vs : 0.f;
         const int exponent = cache_exponent(scale);
         bool todo = held;
         while (__builtin_amdgcn_ballot_w64(todo) != 0) {    // (no page: alpha is 1, or there is nothing yet)
+            anew();
             const int least = cache_over_rows(todo ? exponent : 128, [](int a, int b) { return min(a, b); });
-            const bool use = todo && exponent <= least + kPBits;
+            const bool use = todo && exponent <= least + kSpread;
             // (what is summed must not overflow: the unit stays within 2^80 of its highest)
             const int now = max(cache_over_rows(use ? exponent : -126, [](int a, int b) { return max(a, b); }), peak - 80);
-            const float weight = use ? __builtin_amdgcn_ldexpf(scale, kPBits - exponent) : 0.f;
-            const float vscale = __builtin_amdgcn_ldexpf(1.f, use ? exponent - now : 0);
-            cf16x8_t ph[QB][PT][2];
-#pragma unroll
-            for (int b = 0; b < QB; ++b) {
-                const int seen = held ? limit[b] - vkey : 0;
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    // (the weight of a page that the row does not see may be anything)
-                    const float x = e < seen ? s[b][e / 4][e % 4] * weight : 0.f;
-                    _Float16 terms[PT];
-                    cache_terms<PT>(x, terms);
-#pragma unroll
-                    for (int i = 0; i < PT; ++i) ph[b][i][e / 8][e % 8] = terms[i];
-                }
-                const float rescale = __builtin_amdgcn_ldexpf(alpha[b], unit - now);
-                alpha[b] = 1.f;
-#pragma unroll
-                for (int i = 0; i < NB; ++i) o[b][i] *= rescale;
-            }
-            unit = now;
-            peak = max(peak, now);
+            add<true>(s, alpha, use ? __builtin_amdgcn_ldexpf(scale, kPBits - now) : 0.f, now, seen, values);
             todo = todo && !use;
 #pragma unroll
-            for (int i = 0; i < NB; ++i)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const CacheCodes x = values(i, h);
-                    const uint32_t lo = x.lo & clear[2 * h], hi = x.hi & clear[2 * h + 1];
-                    const uint32_t bad = cache_nan_bytes(lo), bad2 = cache_nan_bytes(hi);
-                    nans |= bad | bad2;
-                    const cf16x8_t a = cache_frag<cf16x8_t>(lo & ~(bad | (bad - (bad >> 7))), hi & ~(bad2 | (bad2 - (bad2 >> 7))), vscale);
-#pragma unroll
-                    for (int j = PT - 1; j >= 0; --j)
-#pragma unroll
-                        for (int b = 0; b < QB; ++b) o[b][i] = cache_mfma(a, ph[b][j][h], o[b][i]);
-                }
+            for (int b = 0; b < QB; ++b) alpha[b] = 1.f;
         }
     }
 
@@ -463,11 +449,12 @@ struct CacheRows {
     __device__ __forceinline__ bool whole(int key0, bool held, int exponent, int &now) const {
         now = cache_over_rows(exponent, [](int a, int b) { return max(a, b); });
         return key0 + kCacheTile <= first_limit && now >= peak - 80 &&
-               __builtin_amdgcn_ballot_w64(!held || exponent < now - kPBits) == 0;
+               __builtin_amdgcn_ballot_w64(!held || exponent < now - kSpread) == 0;
     }
 
-    // After the tiles tile, tile + step, ... below end: o in units of 1, l of the row,
-    // and NaN to the outputs of the rows that see a NaN value of a masked tile.
+    // After the last tile: o in units of 1, l of the row, and NaN to the outputs of
+    // the rows that see a NaN value of step_any()'s tiles: tile, tile + step, ... below
+    // end.
     __device__ __forceinline__ void finish(const CacheAttnParams &p, const CacheItem &it, int tile, int end, int step, int lane) {
 #pragma unroll
         for (int b = 0; b < QB; ++b) {
@@ -481,31 +468,36 @@ struct CacheRows {
         const int g = lane >> 4, r16 = lane & 15, in_page = (1 << p.cache.log2_page) - 1;
         const CacheHead head(p, it);
         for (; tile < end; tile += step) {
-            const int key0 = tile * kCacheTile, vkey = key0 + g * 16;
+            const int vkey = tile * kCacheTile + g * 16;
             const int entry = head.entry(p, vkey);
             const bool held = (uint32_t)entry < (uint32_t)p.cache.pages && vkey < it.keys;
-            if (key0 + kCacheTile <= first_limit && __builtin_amdgcn_ballot_w64(!held) == 0) continue;
             const uint8_t *vp = cache_at(head.v, held ? entry : 0, p.cache.v_sp) + (vkey & in_page) + (int64_t)r16 * p.cache.v_sd;
-            const int any = held ? last_limit - vkey : 0;
+            // bf16 ones where a value is NaN, and where a row sees its token
+            typedef uint32_t words __attribute__((ext_vector_type(4)));
+            words see[QB][2];
+#pragma unroll
+            for (int b = 0; b < QB; ++b) {
+                const int seen = held ? limit[b] - vkey : 0;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) see[b][j / 4][j % 4] = (seen > 2 * j ? 0x3f80u : 0u) | (seen > 2 * j + 1 ? 0x3f800000u : 0u);
+            }
 #pragma unroll
             for (int i = 0; i < NB; ++i) {
                 const uint4 x = *(const uint4 *)(vp + (int64_t)i * 16 * p.cache.v_sd);
                 const uint32_t v[4] = {x.x, x.y, x.z, x.w};
-                cbf16x8_t bad[2];
+                words bad[2];
 #pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    bad[e / 8][e % 8] = (__bf16)((cache_nan_bytes(v[e / 4]) >> (8 * (e % 4) + 7) & 1) && e < any ? 1.f : 0.f);
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t f = cache_nan_bytes(v[j]) >> 7;
+                    bad[j / 2][j % 2 * 2] = (f & 1 | (f & 0x100) << 8) * 0x3f80u;
+                    bad[j / 2][j % 2 * 2 + 1] = (f >> 16 & 1 | (f & 0x1000000) >> 8) * 0x3f80u;
+                }
 #pragma unroll
                 for (int b = 0; b < QB; ++b) {
-                    const int seen = held ? limit[b] - vkey : 0;
                     cf32x4_t hit{};
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        cbf16x8_t see;
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) see[e] = (__bf16)(8 * h + e < seen ? 1.f : 0.f);
-                        hit = cache_mfma(bad[h], see, hit);
-                    }
+                    for (int h = 0; h < 2; ++h)
+                        hit = cache_mfma(__builtin_bit_cast(cbf16x8_t, bad[h]), __builtin_bit_cast(cbf16x8_t, see[b][h]), hit);
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         if (hit[e] > 0.f) o[b][i][e] = __builtin_nanf("");
@@ -580,7 +572,6 @@ struct CacheWave : CacheRows<T, D, 1> {
             this->load(p, it, lane);
             return;
         }
-        const int begin = tile;
         const CacheHead head(p, it);
         // key 16 (r16 / 4) + r16 % 4 of a tile, columns 16 g ..; column r16, key 16 g
         const uint8_t *kp = head.k + (int64_t)((r16 >> 2) * 16 & in_page) * p.cache.k_st + (r16 & 3) * p.cache.k_st + g * (D >= 64 ? 16 : 8);
@@ -593,19 +584,14 @@ struct CacheWave : CacheRows<T, D, 1> {
         load_keys<NT>(p, head, kp, tile, kentry, ventry);
         load_values<NT>(p, vp, tile, ventry);
         const float c0 = p.scale * 1.44269504088896341f;
-        const auto keys = [&](int t, int k) { return CacheCodes{kr[t][2 * k], kr[t][2 * k + 1]}; };
-        const auto values = [&](int i, int h) { return CacheCodes{vr[i][2 * h], vr[i][2 * h + 1]}; };
+        const auto keys = [&](int t, int k) { return cache_frag<typename Rows::frag>(kr[t][2 * k], kr[t][2 * k + 1]); };
+        const auto values = [&](int i, int h) { return cache_frag<cf16x8_t>(vr[i][2 * h], vr[i][2 * h + 1]); };
         // Whole tiles as long as there are such, then the others.
-        bool any = false;
         for (; tile < end; tile += step) {
             const int vkey = tile * kCacheTile + g * 16;
             const bool held = (uint32_t)ventry < (uint32_t)p.cache.pages && vkey < it.keys;
-            const int exponent = cache_exponent(vs);
             int now;
-            if (!this->whole(tile * kCacheTile, held, exponent, now)) {
-                any = true;
-                break;
-            }
+            if (!this->whole(tile * kCacheTile, held, cache_exponent(vs), now)) break;
             const float c = c0 * ks, scale = vs;
             kentry = knext, ventry = vnext;
             // (always loaded, of a tile there is: joining the value with another
@@ -613,15 +599,21 @@ struct CacheWave : CacheRows<T, D, 1> {
             const int ahead = min(tile + 2 * step, end - 1);
             knext = entry(ahead, r16 >> 2), vnext = entry(ahead, g);
             const bool more = tile + step < end;
-            this->step(c, scale, exponent, now, keys, values,
+            this->step(c, scale, now, keys, values,
                        [&] { if (more) load_keys<NT>(p, head, kp, tile + step, kentry, ventry); });
             if (more) load_values<NT>(p, vp, tile + step, ventry);
         }
-        if (any)
+        const int begin = tile;
+        if (tile < end)
             for (; tile < end; tile += step) {
                 const int vkey = tile * kCacheTile + g * 16;
                 const bool held = (uint32_t)ventry < (uint32_t)p.cache.pages && vkey < it.keys;
-                this->step_any(vkey, held, c0 * ks, vs, keys, values, [] {});
+#pragma unroll
+                for (int i = 0; i < NB; ++i) cache_clear(vr[i], held ? this->last_limit - vkey : 0, this->nans);
+                this->step_any(vkey, held, c0 * ks, vs, keys, values, [&] {
+#pragma unroll
+                    for (int i = 0; i < NB * 4; ++i) asm volatile("" : "+v"(vr[i / 4][i % 4]));
+                });
                 if (tile + step < end) {
                     kentry = knext, ventry = vnext;
                     const int ahead = min(tile + 2 * step, end - 1);
@@ -841,85 +833,103 @@ __global__ __launch_bounds__(256) void cache_attn_join_kernel(CacheAttnParams p)
     }
 }
 
-// Chunks of prompts: a wave has 32 rows and all their tiles, which its workgroup
-// stages in the LDS, as codes, one tile ahead of the products (16 KB at head_dim
-// 128 for 128 rows: the matrix unit works 4 times as long on a tile as the L2
-// takes to bring it).  In the LDS 16-byte pieces change places within a row, by
-// the row's number, so that the 16 rows that a read takes lie in all banks.
+// Chunks of prompts: a workgroup has 128 rows, 32 a wave, and all their tiles.  Its
+// waves load a tile's codes together, while they work on the one before, and put
+// them into the LDS as the operands that the products take: a code is converted
+// once for 128 rows.  In the LDS 16-byte pieces change places within a row, by the
+// row's number, so that the 16 rows that a read takes lie in all banks.
 constexpr int kChunkBlocks = 2, kChunkWaves = 4;
 constexpr int kChunkRows = kCacheRows * kChunkBlocks * kChunkWaves;
 
-template <int D>
+template <typename frag, int D>
 struct CacheStage {
-    static constexpr int KP = D / 16;                  // pieces of a key
-    static constexpr int PIECES = 2 * kCacheTile * KP; // of a tile's keys and values
-    static constexpr int BYTES = PIECES * 16;
-    static constexpr int N = PIECES / (kChunkWaves * 64);   // a thread's
+    static constexpr int KP = D / 16;                       // 16-code pieces of a key (of a column: 4)
+    static constexpr int PIECES = kCacheTile * KP;          // of a tile's keys, and of its values
+    static constexpr int BYTES = 2 * PIECES * 32;           // of the LDS
+    static constexpr int N = PIECES / (kChunkWaves * 64);   // a thread's, of keys and of values (D = 32: the first or the second half has one)
+    static constexpr int M = N > 0 ? N : 1;
 
-    // place of a key's piece, of a column's
+    const uint8_t *kat[M], *vat[M];   // the thread's pieces in a page
+    int32_t kentry[M], ventry[M];     // the pages that the next ones are in
+    uint4 k[M], v[M];
+
+    static __device__ __forceinline__ int piece(int n, int tid) { return N > 0 ? n * kChunkWaves * 64 + tid : tid % PIECES; }
+    // D = 32: half of the threads have keys, the others values
+    static __device__ __forceinline__ bool has_keys(int tid) { return N > 0 || tid < PIECES; }
+    static __device__ __forceinline__ bool has_values(int tid) { return N > 0 || tid >= PIECES; }
+    // what the pieces' numbers in a row are xored with
     static __device__ __forceinline__ int key_swap(int row) {
-        return D == 128 ? (row >> 4 & 3) * 2 + (row >> 1 & 1) : D == 64 ? row >> 4 & 3 : 0;
+        return D == 128 ? (row >> 4 & 3) * 4 + (row & 3) : D == 64 ? (row >> 4 & 3) * 2 + (row >> 1 & 1) : row >> 4 & 3;
     }
-    static __device__ __forceinline__ int value_swap(int d) { return d >> 2 & 3; }
+    static __device__ __forceinline__ int value_swap(int d) { return d >> 1 & 7; }
 
-    int32_t entry[N];    // of the pages that the thread's pieces are in
-
-    // First key of the thread's piece n in a tile, the piece's place being
-    // (n * 4 + wave) * 64 + lane: keys first, then values.
-    static __device__ __forceinline__ bool is_key(int n, int wave) { return (n * kChunkWaves + wave) * 64 < PIECES / 2; }
-    static __device__ __forceinline__ int key_of(int n, int wave, int lane) {
-        const int x = (n * kChunkWaves + wave) * 64 + lane;
-        if (is_key(n, wave)) return x / KP;
-        const int y = x - PIECES / 2;
-        return (y % 4 ^ value_swap(y / 4)) * 16;
-    }
-    __device__ __forceinline__ void look_up(const CacheAttnParams &p, const CacheHead &head, int tile, int wave, int lane) {
-#pragma unroll
-        for (int n = 0; n < N; ++n) entry[n] = head.entry(p, tile * kCacheTile + key_of(n, wave, lane));
-    }
-    // the thread's part of a page, and the loads of a tile into `stage`
-    const uint8_t *at[N];
-    __device__ __forceinline__ void place(const CacheAttnParams &p, const CacheHead &head, int wave, int lane) {
+    __device__ __forceinline__ void place(const CacheAttnParams &p, const CacheHead &head, int tid) {
         const int in_page = (1 << p.cache.log2_page) - 1;
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const int x = (n * kChunkWaves + wave) * 64 + lane, key = key_of(n, wave, lane) & in_page;
-            at[n] = is_key(n, wave) ? head.k + (int64_t)key * p.cache.k_st + (x % KP ^ key_swap(x / KP)) * 16
-                                    : head.v + key + (int64_t)((x - PIECES / 2) / 4) * p.cache.v_sd;
+        for (int n = 0; n < M; ++n) {
+            const int x = piece(n, tid);
+            kat[n] = head.k + (int64_t)(x / KP & in_page) * p.cache.k_st + x % KP * 16;
+            vat[n] = head.v + (x % 4 * 16 & in_page) + (int64_t)(x / 4) * p.cache.v_sd;
         }
     }
-    __device__ __forceinline__ void load(const CacheAttnParams &p, uint8_t *stage, int tile, int wave) const {
+    __device__ __forceinline__ void look_up(const CacheAttnParams &p, const CacheHead &head, int tile, int tid) {
+#pragma unroll
+        for (int n = 0; n < M; ++n) {
+            const int x = piece(n, tid);
+            kentry[n] = head.entry(p, tile * kCacheTile + x / KP);
+            ventry[n] = head.entry(p, tile * kCacheTile + x % 4 * 16);
+        }
+    }
+    __device__ __forceinline__ void load(const CacheAttnParams &p, int tile, int tid) {
         const int first = tile * kCacheTile & (1 << p.cache.log2_page) - 1;
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const bool key = is_key(n, wave);
-            const uint8_t *src = cache_at(at[n], cache_page(p, entry[n]), key ? p.cache.k_sp : p.cache.v_sp) + (uint32_t)(key ? first * p.cache.k_st : first);
-            typedef const __attribute__((address_space(1))) void gvoid;
-            typedef __attribute__((address_space(3))) void lvoid;
-            __builtin_amdgcn_global_load_lds((gvoid *)src, (lvoid *)(stage + (n * kChunkWaves + wave) * 1024), 16, 0, 0);
+        for (int n = 0; n < M; ++n) {
+            if (has_keys(tid)) k[n] = *(const uint4 *)(cache_at(kat[n], cache_page(p, kentry[n]), p.cache.k_sp) + (uint32_t)(first * p.cache.k_st));
+            if (has_values(tid)) v[n] = *(const uint4 *)(cache_at(vat[n], cache_page(p, ventry[n]), p.cache.v_sp) + first);
         }
     }
-    static __device__ __forceinline__ CacheCodes key(const uint8_t *stage, int t, int k, int lane) {
+    // `any`: the tile is for step_any(): values past `limit` or of no page are cleared, and NaN
+    __device__ __forceinline__ void store(const CacheAttnParams &p, const CacheItem &it, uint8_t *stage, int tile, int tid, const int32_t (&entry)[M], bool any,
+                                          int limit, uint32_t &nans) const {
+#pragma unroll
+        for (int n = 0; n < M; ++n) {
+            const int x = piece(n, tid);
+            if (has_keys(tid)) {
+                uint8_t *row = stage + x / KP * (D * 2);
+                const int at = x % KP * 2, swap = key_swap(x / KP);
+                *(frag *)(row + (at ^ swap) * 16) = cache_frag<frag>(k[n].x, k[n].y);
+                *(frag *)(row + (at + 1 ^ swap) * 16) = cache_frag<frag>(k[n].z, k[n].w);
+            }
+            if (has_values(tid)) {
+                uint32_t c[4] = {v[n].x, v[n].y, v[n].z, v[n].w};
+                if (any) {
+                    const int key = tile * kCacheTile + x % 4 * 16;
+                    const bool held = (uint32_t)entry[n] < (uint32_t)p.cache.pages && key < it.keys;
+                    cache_clear(c, held ? limit - key : 0, nans);
+                }
+                uint8_t *row = stage + BYTES / 2 + x / 4 * (kCacheTile * 2);
+                const int at = x % 4 * 2, swap = value_swap(x / 4);
+                *(cf16x8_t *)(row + (at ^ swap) * 16) = cache_frag<cf16x8_t>(c[0], c[1]);
+                *(cf16x8_t *)(row + (at + 1 ^ swap) * 16) = cache_frag<cf16x8_t>(c[2], c[3]);
+            }
+        }
+    }
+    static __device__ __forceinline__ frag key(const uint8_t *stage, int t, int k, int lane) {
         const int g = lane >> 4, r16 = lane & 15, row = (r16 >> 2) * 16 + 4 * t + (r16 & 3);
-        if constexpr (D >= 64) {
-            const uint4 x = *(const uint4 *)(stage + row * D + ((k / 2 * 4 + g) ^ key_swap(row)) * 16);
-            return k % 2 ? CacheCodes{x.z, x.w} : CacheCodes{x.x, x.y};
-        } else {
-            const uint2 x = *(const uint2 *)(stage + row * D + g * 8);
-            return CacheCodes{x.x, x.y};
-        }
+        const int at = D >= 64 ? k / 2 * 8 + g * 2 + k % 2 : g;
+        return *(const frag *)(stage + row * (D * 2) + (at ^ key_swap(row)) * 16);
     }
-    static __device__ __forceinline__ CacheCodes value(const uint8_t *stage, int i, int h, int lane) {
+    static __device__ __forceinline__ cf16x8_t value(const uint8_t *stage, int i, int h, int lane) {
         const int g = lane >> 4, d = i * 16 + (lane & 15);
-        const uint4 x = *(const uint4 *)(stage + BYTES / 2 + d * 64 + (g ^ value_swap(d)) * 16);
-        return h ? CacheCodes{x.z, x.w} : CacheCodes{x.x, x.y};
+        return *(const cf16x8_t *)(stage + BYTES / 2 + d * (kCacheTile * 2) + (g * 2 + h ^ value_swap(d)) * 16);
     }
 };
 
 template <typename T, int D>
-__device__ __forceinline__ void cache_chunk(const CacheAttnParams &p, uint8_t *smem, int i) {
-    using Stage = CacheStage<D>;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
+__device__ __forceinline__ void cache_chunk(const CacheAttnParams &p, uint8_t *smem, int *bad, int i) {
+    using Rows = CacheRows<T, D, kChunkBlocks>;
+    using Stage = CacheStage<typename Rows::frag, D>;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
     const auto blocks = [&](const CacheItem &r) {
         return cache_is_chunk(p, r) ? (int)((cache_rows(p, r) + kChunkRows - 1) / kChunkRows) : 0;
     };
@@ -931,53 +941,88 @@ __device__ __forceinline__ void cache_chunk(const CacheAttnParams &p, uint8_t *s
     it.row0 = row0 + wave * kChunkBlocks * kCacheRows;
     cache_uniform(it);
     const int64_t rows = cache_rows(p, it);
-    const int tiles = (cache_limit(p, it, (int)(min((int64_t)row0 + kChunkRows, rows) - 1) / p.group) + kCacheTile - 1) / kCacheTile;
+    // what the workgroup's last and first row see: waves take the same tiles as whole
+    const int last = cache_limit(p, it, (int)(min((int64_t)row0 + kChunkRows, rows) - 1) / p.group);
+    const int tiles = (last + kCacheTile - 1) / kCacheTile;
 
-    CacheRows<T, D, kChunkBlocks> w;
+    int any = 0;
+    Rows w;
     w.load(p, it, lane);
+    w.first_limit = cache_limit(p, it, row0 / p.group);
+    if (tid == 0) *bad = 0;
     if (tiles > 0) {
         const CacheHead head(p, it);
         const auto entry = [&](int tile) { return head.entry(p, tile * kCacheTile + g * 16); };
-        Stage stage;
-        stage.place(p, head, wave, lane);
-        stage.look_up(p, head, 0, wave, lane);
-        int now = entry(0), next = entry(min(1, tiles - 1));
-        stage.load(p, smem, 0, wave);
-        uint32_t page = cache_page(p, now);
-        float next_ks = *(const float *)cache_at(head.ks, page, p.cache.ks_sp), next_vs = *(const float *)cache_at(head.vs, page, p.cache.vs_sp);
-        stage.look_up(p, head, min(1, tiles - 1), wave, lane);
         const float c0 = p.scale * 1.44269504088896341f;
-        for (int tile = 0; tile < tiles; ++tile) {
-            // this tile's loads have ended, and all waves have done with the other stage
-            __builtin_amdgcn_s_waitcnt(0);
-            __syncthreads();
-            const float ks = next_ks, vs = next_vs;
-            const int key0 = tile * kCacheTile, vkey = key0 + g * 16;
-            const bool held = (uint32_t)now < (uint32_t)p.cache.pages && vkey < it.keys;
-            now = next;
-            if (tile + 1 < tiles) stage.load(p, smem + (tile + 1 & 1) * Stage::BYTES, tile + 1, wave);
-            // (always loaded, of a tile there is: joining the values with others would
-            // wait for the loads here)
-            page = cache_page(p, now);
-            next_ks = *(const float *)cache_at(head.ks, page, p.cache.ks_sp);
-            next_vs = *(const float *)cache_at(head.vs, page, p.cache.vs_sp);
-            const int ahead = min(tile + 2, tiles - 1);
-            stage.look_up(p, head, ahead, wave, lane);
-            next = entry(ahead);
-            if (key0 >= w.last_limit) continue;
-            const uint8_t *codes = smem + (tile & 1) * Stage::BYTES;
-            const auto keys = [&](int t, int k) { return Stage::key(codes, t, k, lane); };
-            const auto values = [&](int i, int h) { return Stage::value(codes, i, h, lane); };
-            const int exponent = cache_exponent(vs);
-            int largest;
-            if (w.whole(key0, held, exponent, largest))
-                w.step(c0 * ks, vs, exponent, largest, keys, values, [] {});
-            else
-                w.step_any(vkey, held, c0 * ks, vs, keys, values, [] {});
+        Stage stage;
+        uint32_t nans = 0;
+        stage.place(p, head, tid);
+        stage.look_up(p, head, 0, tid);
+        int lane_entry = entry(0);
+        stage.load(p, 0, tid);
+        float ks, vs;
+        bool held;
+        int largest;
+        // the lane's scales of a tile, and whether step() does for it
+        const auto inspect = [&](int tile) {
+            const uint32_t page = cache_page(p, lane_entry);
+            ks = *(const float *)cache_at(head.ks, page, p.cache.ks_sp);
+            vs = *(const float *)cache_at(head.vs, page, p.cache.vs_sp);
+            held = (uint32_t)lane_entry < (uint32_t)p.cache.pages && tile * kCacheTile + g * 16 < it.keys;
+        };
+        inspect(0);
+        int32_t ventry[Stage::M];
+#pragma unroll
+        for (int j = 0; j < Stage::M; ++j) ventry[j] = stage.ventry[j];
+        int ahead = min(1, tiles - 1);
+        stage.look_up(p, head, ahead, tid);
+        lane_entry = entry(ahead);
+        bool whole = w.whole(0, held, cache_exponent(vs), largest);
+        stage.store(p, it, smem, 0, tid, ventry, !whole, last, nans);
+        int tile = 0;
+        // the workgroup's share in the next tile's stage, before and after a tile's products
+        const auto before = [&] {
+            __syncthreads();    // the tile is there, and the other half is free
+            if (tile + 1 < tiles) stage.load(p, tile + 1, tid);
+#pragma unroll
+            for (int j = 0; j < Stage::M; ++j) ventry[j] = stage.ventry[j];
+            inspect(min(tile + 1, tiles - 1));
+            ahead = min(tile + 2, tiles - 1);
+            stage.look_up(p, head, ahead, tid);
+            lane_entry = entry(ahead);
+        };
+        const auto after = [&] {
+            if (tile + 1 < tiles) {
+                whole = whole && w.whole((tile + 1) * kCacheTile, held, cache_exponent(vs), largest);
+                stage.store(p, it, smem + (tile + 1 & 1) * Stage::BYTES, tile + 1, tid, ventry, !whole, last, nans);
+            }
+        };
+        const auto keys = [&](int t, int k) { return Stage::key(smem + (tile & 1) * Stage::BYTES, t, k, lane); };
+        const auto values = [&](int i, int h) { return Stage::value(smem + (tile & 1) * Stage::BYTES, i, h, lane); };
+        // Whole tiles as long as there are such, then the others.
+        for (; tile < tiles && whole; ++tile) {
+            const float c = c0 * ks, scale = vs;
+            const int now = largest;
+            before();
+            w.step(c, scale, now, keys, values, [] {});
+            after();
         }
+        const int begin = tile;
+        for (; tile < tiles; ++tile) {
+            const float c = c0 * ks, scale = vs;
+            const bool here = held;
+            before();
+            if (tile * kCacheTile < w.last_limit)
+                w.step_any(tile * kCacheTile + g * 16, here, c, scale, keys, values, [] { asm volatile("" ::: "memory"); });
+            after();
+        }
+        if (nans) *bad = 1;
+        __syncthreads();
+        w.nans = *bad;
+        any = begin;
     }
     if (it.row0 >= rows) return;
-    w.finish(p, it, 0, (w.last_limit + kCacheTile - 1) / kCacheTile, 1, lane);
+    w.finish(p, it, any, (w.last_limit + kCacheTile - 1) / kCacheTile, 1, lane);
 #pragma unroll
     for (int b = 0; b < kChunkBlocks; ++b) {
         const int r = b * kCacheRows + (lane & 15);
@@ -993,12 +1038,13 @@ __device__ __forceinline__ void cache_chunk(const CacheAttnParams &p, uint8_t *s
 template <typename T, int D>
 __global__ __launch_bounds__(kChunkWaves * 64, 2) void cache_attn_mixed_kernel(CacheAttnParams p) {
     static_assert(kSplitWaves == kChunkWaves, "one workgroup shape");
-    __shared__ __attribute__((aligned(16))) uint8_t smem[2 * CacheStage<D>::BYTES];
+    __shared__ __attribute__((aligned(16))) uint8_t smem[2 * CacheStage<typename CacheQuery<T>::frag, D>::BYTES];
+    __shared__ int bad;
     const int split = p.ranges / kSplitWaves;
     if ((int)blockIdx.x < split)
         cache_split<T, D>(p, blockIdx.x * kSplitWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), p.ranges);
     else
-        cache_chunk<T, D>(p, smem, blockIdx.x - split);
+        cache_chunk<T, D>(p, smem, &bad, blockIdx.x - split);
 }
 
 }  // namespace pmkl_amd
