@@ -838,7 +838,7 @@ __global__ __launch_bounds__(256) void cache_attn_join_kernel(CacheAttnParams p)
 // them into the LDS as the operands that the products take: a code is converted
 // once for 128 rows.  In the LDS 16-byte pieces change places within a row, by the
 // row's number, so that the 16 rows that a read takes lie in all banks.
-constexpr int kChunkBlocks = 2, kChunkWaves = 4;
+constexpr int kChunkBlocks = 1, kChunkWaves = 8;
 constexpr int kChunkRows = kCacheRows * kChunkBlocks * kChunkWaves;
 
 template <typename frag, int D>
@@ -846,7 +846,7 @@ struct CacheStage {
     static constexpr int KP = D / 16;                       // 16-code pieces of a key (of a column: 4)
     static constexpr int PIECES = kCacheTile * KP;          // of a tile's keys, and of its values
     static constexpr int BYTES = 2 * PIECES * 32;           // of the LDS
-    static constexpr int N = PIECES / (kChunkWaves * 64);   // a thread's, of keys and of values (D = 32: the first or the second half has one)
+    static constexpr int N = PIECES / (kChunkWaves * 64);   // a thread's, of keys and of values; 0: the first PIECES threads have keys, the next values
     static constexpr int M = N > 0 ? N : 1;
 
     const uint8_t *kat[M], *vat[M];   // the thread's pieces in a page
@@ -854,14 +854,17 @@ struct CacheStage {
     uint4 k[M], v[M];
 
     static __device__ __forceinline__ int piece(int n, int tid) { return N > 0 ? n * kChunkWaves * 64 + tid : tid % PIECES; }
-    // D = 32: half of the threads have keys, the others values
     static __device__ __forceinline__ bool has_keys(int tid) { return N > 0 || tid < PIECES; }
-    static __device__ __forceinline__ bool has_values(int tid) { return N > 0 || tid >= PIECES; }
-    // what the pieces' numbers in a row are xored with
+    static __device__ __forceinline__ bool has_values(int tid) { return N > 0 || (tid >= PIECES && tid < 2 * PIECES); }
+    // What the pieces' numbers in a row are xored with.  A read of 16 bytes a lane
+    // serves 16 lanes at a time, which are rows 0 - 3 and 12 - 15 of one piece and
+    // 4 - 11 of the next, or the other way round; these lie in 16 places.
+    static __device__ __forceinline__ int swap8(int i) { return i & 4 | (i & 1) << 1 | (i >> 1 ^ i >> 2) & 1; }
     static __device__ __forceinline__ int key_swap(int row) {
-        return D == 128 ? (row >> 4 & 3) * 4 + (row & 3) : D == 64 ? (row >> 4 & 3) * 2 + (row >> 1 & 1) : row >> 4 & 3;
+        const int a = row >> 4 & 3;
+        return D == 128 ? a * 4 + (row & 3) : D == 64 ? swap8(a * 2 + (row >> 1 & 1)) : (a >> 1 ^ a & 1) << 1 | a >> 1;
     }
-    static __device__ __forceinline__ int value_swap(int d) { return d >> 1 & 7; }
+    static __device__ __forceinline__ int value_swap(int d) { return swap8(d >> 1 & 7); }
 
     __device__ __forceinline__ void place(const CacheAttnParams &p, const CacheHead &head, int tid) {
         const int in_page = (1 << p.cache.log2_page) - 1;
@@ -914,14 +917,29 @@ struct CacheStage {
             }
         }
     }
-    static __device__ __forceinline__ frag key(const uint8_t *stage, int t, int k, int lane) {
-        const int g = lane >> 4, r16 = lane & 15, row = (r16 >> 2) * 16 + 4 * t + (r16 & 3);
-        const int at = D >= 64 ? k / 2 * 8 + g * 2 + k % 2 : g;
-        return *(const frag *)(stage + row * (D * 2) + (at ^ key_swap(row)) * 16);
+};
+
+// Where a lane reads its operands in a stage.
+template <typename frag, int D>
+struct CacheTaker {
+    using Stage = CacheStage<frag, D>;
+    int key_at[D / 32], value_at[2];
+    __device__ __forceinline__ explicit CacheTaker(int lane) {
+        const int g = lane >> 4, r16 = lane & 15, row = (r16 >> 2) * 16 + (r16 & 3);
+#pragma unroll
+        for (int k = 0; k < D / 32; ++k) {
+            const int at = D >= 64 ? k / 2 * 8 + g * 2 + k % 2 : g;
+            key_at[k] = row * (D * 2) + (at ^ Stage::key_swap(row)) * 16;     // (4 rows on: the same swap)
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            value_at[h] = Stage::BYTES / 2 + r16 * (kCacheTile * 2) + (g * 2 + h ^ Stage::value_swap(r16)) * 16;
     }
-    static __device__ __forceinline__ cf16x8_t value(const uint8_t *stage, int i, int h, int lane) {
-        const int g = lane >> 4, d = i * 16 + (lane & 15);
-        return *(const cf16x8_t *)(stage + BYTES / 2 + d * (kCacheTile * 2) + (g * 2 + h ^ value_swap(d)) * 16);
+    __device__ __forceinline__ frag key(const uint8_t *stage, int t, int k) const {
+        return *(const frag *)(stage + key_at[k] + t * (4 * D * 2));
+    }
+    __device__ __forceinline__ cf16x8_t value(const uint8_t *stage, int i, int h) const {
+        return *(const cf16x8_t *)(stage + value_at[h] + i * (16 * kCacheTile * 2));
     }
 };
 
@@ -997,8 +1015,9 @@ __device__ __forceinline__ void cache_chunk(const CacheAttnParams &p, uint8_t *s
                 stage.store(p, it, smem + (tile + 1 & 1) * Stage::BYTES, tile + 1, tid, ventry, !whole, last, nans);
             }
         };
-        const auto keys = [&](int t, int k) { return Stage::key(smem + (tile & 1) * Stage::BYTES, t, k, lane); };
-        const auto values = [&](int i, int h) { return Stage::value(smem + (tile & 1) * Stage::BYTES, i, h, lane); };
+        const CacheTaker<typename Rows::frag, D> taker(lane);
+        const auto keys = [&](int t, int k) { return taker.key(smem + (tile & 1) * Stage::BYTES, t, k); };
+        const auto values = [&](int i, int h) { return taker.value(smem + (tile & 1) * Stage::BYTES, i, h); };
         // Whole tiles as long as there are such, then the others.
         for (; tile < tiles && whole; ++tile) {
             const float c = c0 * ks, scale = vs;
@@ -1033,18 +1052,11 @@ __device__ __forceinline__ void cache_chunk(const CacheAttnParams &p, uint8_t *s
     }
 }
 
-// Both forms in one launch: first the ranges of the requests with few rows, then
-// the chunks.
 template <typename T, int D>
-__global__ __launch_bounds__(kChunkWaves * 64, 2) void cache_attn_mixed_kernel(CacheAttnParams p) {
-    static_assert(kSplitWaves == kChunkWaves, "one workgroup shape");
+__global__ __launch_bounds__(kChunkWaves * 64, kChunkWaves / 2) void cache_attn_chunk_kernel(CacheAttnParams p) {
     __shared__ __attribute__((aligned(16))) uint8_t smem[2 * CacheStage<typename CacheQuery<T>::frag, D>::BYTES];
     __shared__ int bad;
-    const int split = p.ranges / kSplitWaves;
-    if ((int)blockIdx.x < split)
-        cache_split<T, D>(p, blockIdx.x * kSplitWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), p.ranges);
-    else
-        cache_chunk<T, D>(p, smem, &bad, blockIdx.x - split);
+    cache_chunk<T, D>(p, smem, &bad, blockIdx.x);
 }
 
 }  // namespace pmkl_amd

@@ -265,13 +265,13 @@ constexpr int64_t kChunkRows = pmkl_amd::kChunkRows;
 constexpr int64_t kWholeKeys = 1024;
 
 struct AttnKernels {
-    cache_attn_fn whole, split, mixed, join;
+    cache_attn_fn whole, split, chunk, join;
 };
 
 template <typename T, int D>
 AttnKernels attn_kernels() {
     return {pmkl_amd::cache_attn_kernel<T, D, kAttnWaves>, pmkl_amd::cache_attn_split_kernel<T, D>,
-            pmkl_amd::cache_attn_mixed_kernel<T, D>, pmkl_amd::cache_attn_join_kernel<T, D>};
+            pmkl_amd::cache_attn_chunk_kernel<T, D>, pmkl_amd::cache_attn_join_kernel<T, D>};
 }
 template <typename T>
 AttnKernels pick_attn(int64_t D) {
@@ -284,8 +284,9 @@ AttnKernels pick_attn(int64_t D) {
 
 struct AttnPlan {
     AttnKernels fn;
-    bool split, mixed;   // (mixed: split too)
-    int64_t grid, ranges;
+    bool split;
+    int64_t grid, threads, ranges;
+    int64_t chunks;   // workgroups of the chunks' form, beside the split one; 0: it is not used
     uint64_t parts, workspace;   // bytes: of the split form's parts, in all
     bool empty;
 };
@@ -321,21 +322,22 @@ int plan_attn(const pmkl_cache_attn_args *a, AttnPlan *pl) {
     // the split form counts tiles of all row blocks in 32 bits
     const int64_t tiles = (a->table_width * a->cache.page_size + pmkl_amd::kCacheTile - 1) / pmkl_amd::kCacheTile +
                           pmkl_amd::kBlockCost;
+    pl->threads = kAttnWaves * 64;
     pl->split = a->table_width * a->cache.page_size > kWholeKeys && pl->grid <= INT32_MAX / tiles;
     if (pl->split) {
         // as many waves as the chip's 1,024 SIMDs hold of the kernel
-        const int64_t heads = a->cache.kv_heads, rows = a->tokens * G;
-        pl->mixed = rows * heads >= kChunkRows * 256;
-        pl->ranges = 1024 * (D >= 128 || pl->mixed ? 2 : 3);
+        pl->ranges = 1024 * (D >= 128 ? 2 : 3);
         pl->grid = pl->ranges / pmkl_amd::kSplitWaves;
+        pl->threads = pmkl_amd::kSplitWaves * 64;
         pl->parts = (uint64_t)2 * pl->ranges * pmkl_amd::kCacheRows * (D + 2) * sizeof(float);
         pl->workspace = pl->parts + pl->ranges * sizeof(pmkl_amd::CacheUnfinished);
         // enough rows for a workgroup of 128 on every CU: chunks in their own form
-        if (pl->mixed)
-            pl->grid += (rows / kChunkRows + std::min(std::min(a->batch, a->tokens), rows / pmkl_amd::kChunkFrom)) * heads;
+        const int64_t heads = a->cache.kv_heads, rows = a->tokens * G;
+        if (rows * heads >= kChunkRows * 256)
+            pl->chunks = (rows / kChunkRows + std::min(std::min(a->batch, a->tokens), rows / pmkl_amd::kChunkFrom)) * heads;
     }
-    PMKL_REQUIRE(pl->grid * kAttnWaves * 64 < (int64_t(1) << 32), PMKL_EINVAL, "grid too large (%lld workgroups)",
-                 (long long)pl->grid);
+    PMKL_REQUIRE(pl->grid * pl->threads < (int64_t(1) << 32) && pl->chunks * pmkl_amd::kChunkWaves * 64 < (int64_t(1) << 32),
+                 PMKL_EINVAL, "grid too large (%lld workgroups)", (long long)std::max(pl->grid, pl->chunks));
     return PMKL_OK;
 }
 
@@ -383,11 +385,15 @@ int run_attn(const pmkl_cache_attn_args *a, void *stream) {
     p.is_causal = a->is_causal ? 1 : 0;
     p.scale = a->scale > 0.f ? a->scale : 1.0f / std::sqrt((float)D);
     p.ranges = (int32_t)pl.ranges;
-    p.chunks = pl.mixed ? 1 : 0;
-    hipLaunchKernelGGL(pl.mixed ? pl.fn.mixed : pl.split ? pl.fn.split : pl.fn.whole, dim3((unsigned)pl.grid), dim3(kAttnWaves * 64), 0,
+    p.chunks = pl.chunks ? 1 : 0;
+    hipLaunchKernelGGL(pl.split ? pl.fn.split : pl.fn.whole, dim3((unsigned)pl.grid), dim3((unsigned)pl.threads), 0,
                        (hipStream_t)stream, p);
     PMKL_TRY(launched("cache_attn"));
     if (!pl.split) return PMKL_OK;
+    if (pl.chunks) {
+        hipLaunchKernelGGL(pl.fn.chunk, dim3((unsigned)pl.chunks), dim3(pmkl_amd::kChunkWaves * 64), 0, (hipStream_t)stream, p);
+        PMKL_TRY(launched("cache_attn_chunk"));
+    }
     hipLaunchKernelGGL(pl.fn.join, dim3((unsigned)pl.ranges), dim3(256), 0, (hipStream_t)stream, p);
     return launched("cache_attn_join");
 }
@@ -424,11 +430,14 @@ const char *pmkl_cache_attn_kernel_name(const pmkl_cache_attn_args *a) {
     if (plan_attn(a, &pl) != PMKL_OK) return nullptr;
     if (pl.empty) return "none";
     const char *dt = a->dtype == PMKL_DTYPE_BF16 ? "bf16" : a->dtype == PMKL_DTYPE_F16 ? "fp16" : "fp32";
-    const int n = snprintf(name, sizeof(name), "cache_attn_%skernel<%s, %lld> grid %lld x %d", pl.mixed ? "mixed_" : pl.split ? "split_" : "",
-                           dt, (long long)a->cache.head_dim, (long long)pl.grid, kAttnWaves * 64);
+    const long long D = a->cache.head_dim;
+    int n = snprintf(name, sizeof(name), "cache_attn_%skernel<%s, %lld> grid %lld x %d", pl.split ? "split_" : "", dt, D,
+                     (long long)pl.grid, (int)pl.threads);
+    if (pl.chunks)
+        n += snprintf(name + n, sizeof(name) - n, ", cache_attn_chunk_kernel<%s, %lld> grid %lld x %d", dt, D,
+                      (long long)pl.chunks, pmkl_amd::kChunkWaves * 64);
     if (pl.split)
-        snprintf(name + n, sizeof(name) - n, ", cache_attn_join_kernel<%s, %lld> grid %lld x 256", dt,
-                 (long long)a->cache.head_dim, (long long)pl.ranges);
+        snprintf(name + n, sizeof(name) - n, ", cache_attn_join_kernel<%s, %lld> grid %lld x 256", dt, D, (long long)pl.ranges);
     return name;
 }
 

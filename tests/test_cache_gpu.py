@@ -169,7 +169,8 @@ def _form(cache, q):
                                   dtype={2: capi.PMKL_DTYPE_BF16, 4: capi.PMKL_DTYPE_F32}[q.element_size()],
                                   tokens=q.shape[0], heads=q.shape[1], batch=cache.table.shape[0],
                                   table_width=cache.table.shape[1])
-    return capi.cache_attn_kernel_name(a).split("_kernel")[0]
+    names = capi.cache_attn_kernel_name(a)
+    return "chunk" if "_chunk_" in names else "split" if "_split_" in names else "whole"
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
@@ -190,7 +191,7 @@ def test_chunks(device, dtype, dim, page, kv_heads, group, causal):
     cache.v_scale[cache.table[5, -(-65 // page) - 1]] *= 2.0 ** -30
     cache.refresh()
     q = _q(sum(new) + 10, kv_heads * group, dim, dtype, seed=dim)
-    assert _form(cache, q) == "cache_attn_mixed"
+    assert _form(cache, q) == "chunk"
     out, m, l = _attend(cache, q, new, causal=causal, label=f"{dtype} {dim}")
     if causal:
         # request 3: rows 650 .. 949 stand at 340 .. 639
@@ -199,8 +200,7 @@ def test_chunks(device, dtype, dim, page, kv_heads, group, causal):
 
 def test_forms(device):
     """The sizes of these tests reach every form."""
-    for lengths, tokens, heads, form in (([1000], 1, 4, "cache_attn"), ([1100], 1, 4, "cache_attn_split"),
-                                         ([1100], 2000, 32, "cache_attn_mixed")):
+    for lengths, tokens, heads, form in (([1000], 1, 4, "whole"), ([1100], 1, 4, "split"), ([1100], 2000, 32, "chunk")):
         assert _form(Cache(lengths, 2, 16, 64, seed=1, width_more=0), _q(tokens, heads, 64, "bf16", 1)) == form
 
 
