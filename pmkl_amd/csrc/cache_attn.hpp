@@ -217,13 +217,6 @@ __device__ __forceinline__ bool cache_find(const CacheAttnParams &p, int &i, int
     }
     return false;
 }
-template <typename Weight>
-__device__ __forceinline__ int cache_total(const CacheAttnParams &p, int lane, Weight weight) {
-    int sum = 0;
-    for (int b = lane; b < p.batch; b += 64) sum += weight(cache_request(p, b));
-    return __builtin_amdgcn_readlane(wave_scan(sum), 63);
-}
-
 // A head's pages.  Strides between pages are below 2^31 (checked): a page's place
 // is one multiply-add.
 struct CacheHead {
@@ -329,8 +322,9 @@ struct CacheRows {
         }
     }
 
-    // Scores (times c) to weights; alpha: what the sums so far are worth now.
-    __device__ __forceinline__ void weigh(cf32x4_t (&s)[QB][4], float c, float (&alpha)[QB]) {
+    // Scores (times c) to weights, times 2^shift, of which `unshift` is the inverse;
+    // alpha: what the sums so far are worth now.
+    __device__ __forceinline__ void weigh(cf32x4_t (&s)[QB][4], float c, float shift, float unshift, float (&alpha)[QB]) {
 #pragma unroll
         for (int b = 0; b < QB; ++b) {
             float mx = s[b][0][0];
@@ -343,15 +337,15 @@ struct CacheRows {
             float sum = 0.f;
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                const float x = __builtin_amdgcn_exp2f(fmaf(s[b][e / 4][e % 4], c, -ref));
+                const float x = __builtin_amdgcn_exp2f(fmaf(s[b][e / 4][e % 4], c, shift - ref));
                 s[b][e / 4][e % 4] = x;
                 sum += x;
             }
-            l[b] = l[b] * alpha[b] + sum;
+            l[b] = l[b] * alpha[b] + sum * unshift;
         }
     }
 
-    // o = o alpha + P V, P being s times the lane's weight (where seen[b] > e)
+    // o = o alpha + P V, P being s (MASKED: times the lane's weight, where seen[b] > e)
     template <bool MASKED, typename V>
     __device__ __forceinline__ void add(const cf32x4_t (&s)[QB][4], const float (&alpha)[QB], float weight, int now, const int (&seen)[QB], V values) {
         float rescale[QB];
@@ -377,8 +371,8 @@ struct CacheRows {
             for (int b = 0; b < QB; ++b)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    float x = s[b][h * 2 + e / 4][e % 4] * weight;
-                    if (MASKED && h * 8 + e >= seen[b]) x = 0.f;   // (of a page that the row does not see the weight may be anything)
+                    float x = s[b][h * 2 + e / 4][e % 4];
+                    if constexpr (MASKED) x = h * 8 + e < seen[b] ? x * weight : 0.f;   // (of a page that the row does not see the weight may be anything)
                     _Float16 terms[PT];
                     cache_terms<PT>(x, terms);
 #pragma unroll
@@ -405,8 +399,10 @@ struct CacheRows {
         float alpha[QB];
         scores(s, keys);
         taken();
-        weigh(s, c, alpha);
-        add<false>(s, alpha, __builtin_amdgcn_ldexpf(vs, kPBits - now), now, limit, values);
+        // the values' scale, a factor of the lane, goes into the exponent
+        const float weight = __builtin_amdgcn_ldexpf(vs, kPBits - now);
+        weigh(s, c, __builtin_amdgcn_logf(weight), __builtin_amdgcn_rcpf(weight), alpha);
+        add<false>(s, alpha, 1.f, now, limit, values);
     }
 
     // Any other tile; its lane has keys vkey .. vkey + 15, `held` if their page is
@@ -427,7 +423,7 @@ struct CacheRows {
                 s[b][e / 4][e % 4] = e < seen[b] ? x : -INFINITY;
             }
         }
-        weigh(s, 1.f, alpha);
+        weigh(s, 1.f, 0.f, 1.f, alpha);
         // Pages within 2^8 of the least scale take part together, then the others.
         const float scale = held ? vs : 0.f;
         const int exponent = cache_exponent(scale);
@@ -446,10 +442,11 @@ struct CacheRows {
     }
 
     // Whether step() does for a tile, and its largest exponent.
-    __device__ __forceinline__ bool whole(int key0, bool held, int exponent, int &now) const {
+    __device__ __forceinline__ bool whole(int key0, bool held, float scale, int &now) const {
+        const int exponent = cache_exponent(scale);
         now = cache_over_rows(exponent, [](int a, int b) { return max(a, b); });
         return key0 + kCacheTile <= first_limit && now >= peak - 80 &&
-               __builtin_amdgcn_ballot_w64(!held || exponent < now - kSpread) == 0;
+               __builtin_amdgcn_ballot_w64(!(held && scale >= 0x1p-126f && exponent >= now - kSpread)) == 0;
     }
 
     // After the last tile: o in units of 1, l of the row, and NaN to the outputs of
@@ -591,7 +588,7 @@ struct CacheWave : CacheRows<T, D, 1> {
             const int vkey = tile * kCacheTile + g * 16;
             const bool held = (uint32_t)ventry < (uint32_t)p.cache.pages && vkey < it.keys;
             int now;
-            if (!this->whole(tile * kCacheTile, held, cache_exponent(vs), now)) break;
+            if (!this->whole(tile * kCacheTile, held, vs, now)) break;
             const float c = c0 * ks, scale = vs;
             kentry = knext, ventry = vnext;
             // (always loaded, of a tile there is: joining the value with another
@@ -734,15 +731,27 @@ __device__ __forceinline__ int cache_weight(const CacheAttnParams &p, const Cach
 template <typename T, int D>
 __device__ __forceinline__ void cache_split(const CacheAttnParams &p, int range, int ranges) {
     const int lane = threadIdx.x & 63, g = lane >> 4, r16 = lane & 15;
-    const auto weight = [&](const CacheItem &r) { return cache_weight(p, r); };
-    const int total = cache_total(p, lane, weight);
-    const int per = (total + ranges - 1) / ranges;
-    const int lo = (int)min((int64_t)range * per, (int64_t)total), hi = min(lo + per, total);
+    const auto weight = [&](int b) { return b < p.batch ? cache_weight(p, cache_request(p, b)) : 0; };
+    // of the first 64 requests, and of all
+    const int own = weight(lane), sums = wave_scan(own), first = __builtin_amdgcn_readlane(sums, 63);
+    int rest = 0;
+    for (int b = 64 + lane; b < p.batch; b += 64) rest += weight(b);
+    if (p.batch > 64) rest = __builtin_amdgcn_readlane(wave_scan(rest), 63);
+    const int total = first + rest;
+    ranges = min(ranges, total);          // none is empty
+    const auto begin_of = [&](int r) { return (int)((int64_t)r * total / ranges); };
+    const int lo = range < ranges ? begin_of(range) : 0, hi = range < ranges ? begin_of(range + 1) : 0;
     CacheUnfinished left{};
     CacheItem it;
     int i = lo;                           // the place among the request's
     if (lo < hi) {
-        cache_find(p, i, lane, it, weight);
+        if (lo < first) {
+            const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(lo < sums));
+            i -= __builtin_amdgcn_readlane(sums, l) - __builtin_amdgcn_readlane(own, l);
+            it = cache_request(p, l);
+        } else {
+            cache_find(p, i, lane, it, [&](const CacheItem &r) { return cache_weight(p, r); });
+        }
         cache_uniform(it);
     }
     CacheWave<T, D> w;
@@ -759,7 +768,8 @@ __device__ __forceinline__ void cache_split(const CacheAttnParams &p, int range,
             const int number = 2 * range + (at != lo);
             const bool all = from == 0 && end == length;
             if (from == 0 && end < length)
-                left = CacheUnfinished{rows, it.q0, it.head, it.row0, (at - begin + length - 1) / per - range + 1, number, {0, 0}};
+                left = CacheUnfinished{rows, it.q0, it.head, it.row0,
+                                       (int)(((int64_t)(at - begin + length) * ranges - 1) / total) - range + 1, number, {0, 0}};
             float *part = p.parts + (int64_t)number * cache_part_floats<D>();
             if (r16 < rows) {
                 if (all) {
@@ -794,42 +804,91 @@ __global__ __launch_bounds__(kSplitWaves * 64, D >= 128 ? 2 : 3) void cache_attn
     cache_split<T, D>(p, blockIdx.x * kSplitWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), p.ranges);
 }
 
-// Workgroup w adds up the parts of the block that range w leaves unfinished, a row
-// to a wave: D / 4 lanes have the columns of a part.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void cache_attn_join_kernel(CacheAttnParams p) {
-    const CacheUnfinished u = p.unfinished[blockIdx.x];
+// Adds up the parts of the blocks that ranges leave unfinished.  A workgroup looks
+// at PER ranges and takes their blocks one after the other; a row has NW waves,
+// over the rows (a power of two), whose D / 4 lanes have the columns of a part.
+// Parts come from the L2s of other dies, 2 us away: a wave has eight on the way at
+// once, with what they weigh.  Few blocks of many parts: NW 16, PER 8 (64 parts in
+// 4.5 us, by four waves with the largest weight looked up first 14); else a
+// workgroup of four waves for each range.
+template <typename T, int D, int NW, int PER>
+__global__ __launch_bounds__(NW * 64) void cache_attn_join_kernel(CacheAttnParams p) {
+    __shared__ __attribute__((aligned(16))) float share[NW][D];
+    __shared__ float share_m[NW], share_l[NW];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    CacheItem it;
-    it.q0 = u.q0, it.head = u.head, it.row0 = u.row0;
     constexpr int PF = cache_part_floats<D>();
-    const float *first = p.parts + (int64_t)u.first * PF;
-    const float *rest = p.parts + 2 * (int64_t)blockIdx.x * PF;    // part k > 0 is rest[2 k]
-    const auto part = [&](int k) { return k ? rest + (int64_t)2 * k * PF : first; };
-    constexpr int SL = 64 / (D / 4);                                // parts at a time
+    constexpr int SL = 64 / (D / 4);                                // parts of a load
     const int slice = lane / (D / 4), d = lane % (D / 4) * 4;
-    for (int r = wave; r < u.rows; r += 4) {
-        float mx = -INFINITY;
-        for (int k = lane; k < u.parts; k += 64) mx = cache_max(mx, part(k)[kCacheRows * D + r]);
+    int rows[PER];
 #pragma unroll
-        for (int x = 1; x < 64; x <<= 1) mx = cache_max(mx, __shfl_xor(mx, x));
-        const float ref = mx == -INFINITY ? 0.f : mx;
-        float sum = 0.f;
-        cf32x4_t x{};
-#pragma unroll 4
-        for (int k = slice; k < u.parts; k += SL) {
-            const float *q = part(k);
-            const float f = __builtin_amdgcn_exp2f(q[kCacheRows * D + r] - ref);
-            sum += q[kCacheRows * (D + 1) + r] * f;
-            x += *(const cf32x4_t *)(q + r * D + d) * f;
+    for (int j = 0; j < PER; ++j) rows[j] = p.unfinished[blockIdx.x * PER + j].rows;
+    bool used = false;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        if (rows[j] == 0) continue;
+        const int range = blockIdx.x * PER + j;
+        const CacheUnfinished u = p.unfinished[range];
+        CacheItem it;
+        it.q0 = u.q0, it.head = u.head, it.row0 = u.row0;
+        const float *first = p.parts + (int64_t)u.first * PF;
+        const float *rest = p.parts + 2 * (int64_t)range * PF;      // part k > 0 is rest[2 k]
+        const int waves = max(NW >> (32 - __builtin_clz(u.rows) - ((u.rows & (u.rows - 1)) == 0 ? 1 : 0)), 1);   // of a row
+        const int sub = wave % waves;
+        if (used) __syncthreads();                                   // the block before has left the LDS
+        for (int r = wave / waves; r < (waves > 1 ? wave / waves + 1 : u.rows); r += NW / waves) {
+            // (several waves have one row each, and meet below; there may be none for it)
+            float m = -INFINITY, l = 0.f;
+            cf32x4_t x{};
+            for (int k0 = sub * SL + slice; r < u.rows && k0 < u.parts; k0 += SL * waves * 8) {
+                float pm[8], pl[8];
+                cf32x4_t px[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int k = min(k0 + e * SL * waves, u.parts - 1);
+                    const float *part = k ? rest + (int64_t)2 * k * PF : first;
+                    pm[e] = part[kCacheRows * D + r];
+                    pl[e] = part[kCacheRows * (D + 1) + r];
+                    px[e] = *(const cf32x4_t *)(part + r * D + d);
+                }
+                float mx = m;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) mx = cache_max(mx, pm[e]);
+                const float ref = mx == -INFINITY ? 0.f : mx;
+                const float f = __builtin_amdgcn_exp2f(m - ref);
+                m = mx, l *= f, x *= f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (k0 + e * SL * waves < u.parts) {
+                        const float w = __builtin_amdgcn_exp2f(pm[e] - ref);
+                        l += pl[e] * w;
+                        x += px[e] * w;
+                    }
+            }
+            // over the lanes of a column
+            const auto join = [&](float m2, float l2, cf32x4_t x2) {
+                const float mx = cache_max(m, m2), ref = mx == -INFINITY ? 0.f : mx;
+                const float f = __builtin_amdgcn_exp2f(m - ref), f2 = __builtin_amdgcn_exp2f(m2 - ref);
+                m = mx;
+                l = l * f + l2 * f2;
+                x = x * f + x2 * f2;
+            };
+#pragma unroll
+            for (int y = D / 4; y < 64; y <<= 1) {
+                cf32x4_t x2;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x2[e] = __shfl_xor(x[e], y);
+                join(__shfl_xor(m, y), __shfl_xor(l, y), x2);
+            }
+            if (waves > 1) {
+                if (slice == 0) *(cf32x4_t *)&share[wave][d] = x;
+                if (lane == 0) share_m[wave] = m, share_l[wave] = l;
+                __syncthreads();
+                used = true;
+                if (sub == 0)
+                    for (int w = 1; w < waves; ++w) join(share_m[wave + w], share_l[wave + w], *(const cf32x4_t *)&share[wave + w][d]);
+            }
+            if (sub == 0 && slice == 0 && r < u.rows) cache_store<T, D>(p, it, r, d, x, m, l);
         }
-#pragma unroll
-        for (int y = D / 4; y < 64; y <<= 1) {
-            sum += __shfl_xor(sum, y);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] += __shfl_xor(x[e], y);
-        }
-        if (slice == 0) cache_store<T, D>(p, it, r, d, x, mx, sum);
     }
 }
 
@@ -995,7 +1054,7 @@ __device__ __forceinline__ void cache_chunk(const CacheAttnParams &p, uint8_t *s
         int ahead = min(1, tiles - 1);
         stage.look_up(p, head, ahead, tid);
         lane_entry = entry(ahead);
-        bool whole = w.whole(0, held, cache_exponent(vs), largest);
+        bool whole = w.whole(0, held, vs, largest);
         stage.store(p, it, smem, 0, tid, ventry, !whole, last, nans);
         int tile = 0;
         // the workgroup's share in the next tile's stage, before and after a tile's products
@@ -1011,7 +1070,7 @@ __device__ __forceinline__ void cache_chunk(const CacheAttnParams &p, uint8_t *s
         };
         const auto after = [&] {
             if (tile + 1 < tiles) {
-                whole = whole && w.whole((tile + 1) * kCacheTile, held, cache_exponent(vs), largest);
+                whole = whole && w.whole((tile + 1) * kCacheTile, held, vs, largest);
                 stage.store(p, it, smem + (tile + 1 & 1) * Stage::BYTES, tile + 1, tid, ventry, !whole, last, nans);
             }
         };

@@ -248,10 +248,11 @@ int run_append(const pmkl_cache_append_args *a, void *stream) {
     p.kv_heads = (int32_t)H;
     // Of 64 tokens between 64 runs (decoding) and 1 (a prompt in large pages)
     // begin; each is 2 H wave items.  About 8,192 waves in all keep the card
-    // busy, and no more than the items of 64 runs.
+    // busy; more, where a window of a prompt needs them for a page each, and no
+    // more than the items of 64 runs.
     const int64_t windows = (a->tokens + 63) / 64, waves = pmkl_amd::kCacheThreads / 64;
-    const int64_t most = std::min<int64_t>(64, a->tokens) * 2 * H / waves;
-    const int64_t y = std::max<int64_t>(1, std::min(most, 8192 / (windows * waves)));
+    const int64_t runs = std::min<int64_t>(64, a->tokens), pages = std::min<int64_t>(runs, 64 / a->cache.page_size + 1);
+    const int64_t y = std::max<int64_t>({1, std::min(runs * 2 * H, 8192 / windows) / waves, pages * 2 * H / waves});
     const append_fn fn = a->dtype == PMKL_DTYPE_F32 ? pick_append<float>(D)
                          : a->dtype == PMKL_DTYPE_F16 ? pick_append<_Float16>(D) : pick_append<__bf16>(D);
     PMKL_REQUIRE(windows * y * pmkl_amd::kCacheThreads < (int64_t(1) << 32), PMKL_EINVAL, "grid too large");
@@ -264,14 +265,17 @@ constexpr int kAttnWaves = 4;
 constexpr int64_t kChunkRows = pmkl_amd::kChunkRows;
 constexpr int64_t kWholeKeys = 1024;
 
+constexpr int kJoinPer = 8, kJoinWaves = 4;
+
 struct AttnKernels {
-    cache_attn_fn whole, split, chunk, join;
+    cache_attn_fn whole, split, chunk, join, join_many;
 };
 
 template <typename T, int D>
 AttnKernels attn_kernels() {
     return {pmkl_amd::cache_attn_kernel<T, D, kAttnWaves>, pmkl_amd::cache_attn_split_kernel<T, D>,
-            pmkl_amd::cache_attn_chunk_kernel<T, D>, pmkl_amd::cache_attn_join_kernel<T, D>};
+            pmkl_amd::cache_attn_chunk_kernel<T, D>, pmkl_amd::cache_attn_join_kernel<T, D, kJoinWaves, 1>,
+            pmkl_amd::cache_attn_join_kernel<T, D, 16, kJoinPer>};
 }
 template <typename T>
 AttnKernels pick_attn(int64_t D) {
@@ -286,6 +290,7 @@ struct AttnPlan {
     AttnKernels fn;
     bool split;
     int64_t grid, threads, ranges;
+    bool join_many;   // blocks of many parts
     int64_t chunks;   // workgroups of the chunks' form, beside the split one; 0: it is not used
     uint64_t parts, workspace;   // bytes: of the split form's parts, in all
     bool empty;
@@ -325,12 +330,15 @@ int plan_attn(const pmkl_cache_attn_args *a, AttnPlan *pl) {
     pl->threads = kAttnWaves * 64;
     pl->split = a->table_width * a->cache.page_size > kWholeKeys && pl->grid <= INT32_MAX / tiles;
     if (pl->split) {
+        const int64_t blocks = pl->grid;
         // as many waves as the chip's 1,024 SIMDs hold of the kernel
         pl->ranges = 1024 * (D >= 128 ? 2 : 3);
         pl->grid = pl->ranges / pmkl_amd::kSplitWaves;
         pl->threads = pmkl_amd::kSplitWaves * 64;
         pl->parts = (uint64_t)2 * pl->ranges * pmkl_amd::kCacheRows * (D + 2) * sizeof(float);
         pl->workspace = pl->parts + pl->ranges * sizeof(pmkl_amd::CacheUnfinished);
+        // at most so many blocks have parts, and all of them together few more parts than ranges
+        pl->join_many = blocks * 24 < pl->ranges;
         // enough rows for a workgroup of 128 on every CU: chunks in their own form
         const int64_t heads = a->cache.kv_heads, rows = a->tokens * G;
         if (rows * heads >= kChunkRows * 256)
@@ -394,7 +402,10 @@ int run_attn(const pmkl_cache_attn_args *a, void *stream) {
         hipLaunchKernelGGL(pl.fn.chunk, dim3((unsigned)pl.chunks), dim3(pmkl_amd::kChunkWaves * 64), 0, (hipStream_t)stream, p);
         PMKL_TRY(launched("cache_attn_chunk"));
     }
-    hipLaunchKernelGGL(pl.fn.join, dim3((unsigned)pl.ranges), dim3(256), 0, (hipStream_t)stream, p);
+    if (pl.join_many)
+        hipLaunchKernelGGL(pl.fn.join_many, dim3((unsigned)pl.ranges / kJoinPer), dim3(1024), 0, (hipStream_t)stream, p);
+    else
+        hipLaunchKernelGGL(pl.fn.join, dim3((unsigned)pl.ranges), dim3(kJoinWaves * 64), 0, (hipStream_t)stream, p);
     return launched("cache_attn_join");
 }
 
@@ -437,7 +448,9 @@ const char *pmkl_cache_attn_kernel_name(const pmkl_cache_attn_args *a) {
         n += snprintf(name + n, sizeof(name) - n, ", cache_attn_chunk_kernel<%s, %lld> grid %lld x %d", dt, D,
                       (long long)pl.chunks, pmkl_amd::kChunkWaves * 64);
     if (pl.split)
-        snprintf(name + n, sizeof(name) - n, ", cache_attn_join_kernel<%s, %lld> grid %lld x 256", dt, D, (long long)pl.ranges);
+        snprintf(name + n, sizeof(name) - n, ", cache_attn_join_kernel<%s, %lld, %d, %d> grid %lld x %d", dt, D,
+                 pl.join_many ? 16 : kJoinWaves, pl.join_many ? kJoinPer : 1, (long long)(pl.join_many ? pl.ranges / kJoinPer : pl.ranges),
+                 pl.join_many ? 1024 : kJoinWaves * 64);
     return name;
 }
 

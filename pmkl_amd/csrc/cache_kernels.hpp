@@ -153,21 +153,28 @@ __device__ __forceinline__ float cache_scale_for(float a) {
     return __uint_as_float((uint32_t)max(e, 1) << 23);
 }
 
-// x / s as an e4m3 operand: s is a power of two unless the caller made it.  What
-// is not finite becomes NaN (e4m3 has no infinity, and 448 in its place would
-// hide it).
+// x / s as an e4m3 operand.  s is a power of two unless the caller made it: then
+// x (1 / s) is the same.  What is not finite becomes NaN (e4m3 has no infinity,
+// and 448 in its place would hide it).
+template <bool POWER>
 struct CacheQuotient {
-    float s, inverse;
-    bool exact;
-    __device__ explicit CacheQuotient(float scale) : s(scale) {
-        exact = (__float_as_uint(s) & 0x7fffff) == 0 && s >= 0x1p-126f;
-        inverse = 1.f / s;   // of a power of two in 2^-126 .. 2^127: exact
-    }
-    __device__ float operator()(float x) const {
-        const float y = exact ? x * inverse : x / s;
+    float s;      // POWER: its inverse, exact for 2^-126 .. 2^127
+    __device__ explicit CacheQuotient(float scale) : s(POWER ? 1.f / scale : scale) {}
+    __device__ __forceinline__ float operator()(float x) const {
+        const float y = POWER ? x * s : x / s;
         return fabsf(x) < INFINITY ? y : __builtin_nanf("");
     }
 };
+__device__ __forceinline__ bool is_power(float s) { return (__float_as_uint(s) & 0x7fffff) == 0 && s >= 0x1p-126f; }
+
+// f(CacheQuotient) for a scale that is the same in the wave
+template <typename F>
+__device__ __forceinline__ void with_quotient(float scale, F f) {
+    if (is_power(scale))
+        f(CacheQuotient<true>(scale));
+    else
+        f(CacheQuotient<false>(scale));
+}
 
 template <typename T, int N>
 struct alignas(sizeof(T) * N) CacheVec {
@@ -185,6 +192,34 @@ __device__ __forceinline__ float finite_max(const CacheVec<T, N> &x, float a) {
     return a;
 }
 
+// N elements as they were loaded: whole words, where the elements by themselves
+// would take a register each.  settle() keeps what was made of them (their fp32
+// values) from being held beside them.
+template <typename T, int N>
+struct CacheRaw {
+    static constexpr int W = sizeof(T) * N / 4;
+    typedef uint32_t words __attribute__((ext_vector_type(W)));
+    words w;
+    __device__ __forceinline__ void load(const T *p) { w = *(const words *)p; }
+    __device__ __forceinline__ CacheVec<T, N> get() const { return __builtin_bit_cast(CacheVec<T, N>, w); }
+    __device__ __forceinline__ void settle() { asm volatile("" : "+v"(w)); }
+};
+template <typename T>
+struct CacheRaw<T, 2> {
+    static constexpr int W = sizeof(T) * 2 / 4;
+    uint32_t w[W];
+    __device__ __forceinline__ void load(const T *p) {
+        const CacheVec<uint32_t, W> x = *(const CacheVec<uint32_t, W> *)p;
+#pragma unroll
+        for (int i = 0; i < W; ++i) w[i] = x.v[i];
+    }
+    __device__ __forceinline__ CacheVec<T, 2> get() const { return __builtin_bit_cast(CacheVec<T, 2>, w); }
+    __device__ __forceinline__ void settle() {
+#pragma unroll
+        for (int i = 0; i < W; ++i) asm volatile("" : "+v"(w[i]));
+    }
+};
+
 // codes of a dword times f
 __device__ __forceinline__ uint32_t cache_rescale(uint32_t codes, float f) {
     const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(codes, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(codes, true);
@@ -200,14 +235,17 @@ __device__ __forceinline__ uint32_t byte_mask(int at, int from, int to) {
 }
 
 // A wave owns (run, head, keys or values): it reads the run's rows for their
-// largest value, then again, out of the caches, for the codes.  A workgroup's
-// waves, and blockIdx.y's of the same 64 tokens, share what runs begin among
-// these tokens: runs are found on the spot, so the call needs neither the
+// largest value and makes the codes of them, from the registers where they fit (a
+// run inside one page of 16 or 32), else read again, out of the caches.  A
+// workgroup's waves, and blockIdx.y's of the same 64 tokens, share what runs begin
+// among these tokens: runs are found on the spot, so the call needs neither the
 // requests nor their lengths.  Values are transposed on the way: a lane has two
 // columns and 16 tokens of a page, and stores each column's 16 codes as one
 // vector, with the codes around the run read first.
+constexpr int kAppendRows = 8;   // vectors of a lane that are kept
+
 template <typename T, int D>
-__global__ __launch_bounds__(kCacheThreads) void cache_append_kernel(AppendParams p) {
+__global__ __launch_bounds__(kCacheThreads, 4) void cache_append_kernel(AppendParams p) {
     constexpr int E = 16 / (int)sizeof(T);      // elements of a vector
     constexpr int LPR = D / E;                    // lanes of a row
     const int lane = threadIdx.x & 63;
@@ -244,69 +282,150 @@ __global__ __launch_bounds__(kCacheThreads) void cache_append_kernel(AppendParam
             n += 64;
         }
 
+        const float *scale = which ? p.cache.v_scale + page * (p.cache.vs_sp / 4) + head * p.cache.vs_sh
+                                   : p.cache.k_scale + page * (p.cache.ks_sp / 4) + head * p.cache.ks_sh;
+        const float was = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(*scale)));
         const int64_t st = which ? p.v_st : p.k_st;
         const T *x = which ? (const T *)p.v + t0 * p.v_st + head * p.v_sh : (const T *)p.k + t0 * p.k_st + head * p.k_sh;
-        float a = 0.f;
-        for (int i = lane / LPR; i < n; i += 64 / LPR)
-            a = finite_max(*(const CacheVec<T, E> *)(x + i * st + lane % LPR * E), a);
-        a = wave_max(a);
-
-        float *scale = which ? p.cache.v_scale + page * (p.cache.vs_sp / 4) + head * p.cache.vs_sh
-                             : p.cache.k_scale + page * (p.cache.ks_sp / 4) + head * p.cache.ks_sh;
-        const float was = *scale, need = cache_scale_for(a);
-        const bool kept = o > 0 && was > 0.f && was < INFINITY;
-        const float now = kept ? fmaxf(was, need) : need;
-        const bool grown = kept && now != was;
-        const float shrink = was / now;
-        const CacheQuotient quotient(now);
-        if (lane == 0 && !(kept && now == was)) *scale = now;
-
+        // The new scale, and what it is of.
+        float now = 0.f;
+        bool grown = false;
+        const auto rescale = [&](float a) {
+            const float need = cache_scale_for(__uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(wave_max(a)))));
+            const bool kept = o > 0 && was > 0.f && was < INFINITY;
+            now = kept ? fmaxf(was, need) : need;
+            grown = kept && now != was;
+            if (lane == 0 && !(kept && now == was)) *const_cast<float *>(scale) = now;
+        };
+        typedef CacheRaw<T, E> Row;
+        constexpr int RPI = 64 / LPR;             // rows at a time
+        const T *at = x + lane % LPR * E;
+        const auto row_at = [&](int i) {           // past the last: the last
+            Row r;
+            r.load(at + min(i, n - 1) * st);
+            return r;
+        };
         if (which == 0) {
             uint8_t *k = p.cache.k + page * p.cache.k_sp + head * p.cache.k_sh;
-            for (int i = lane / LPR; i < n; i += 64 / LPR) {
-                const auto r = *(const CacheVec<T, E> *)(x + i * st + lane % LPR * E);
+            const auto store = [&](const Row &raw, int i, const auto &quotient) {
+                const auto r = raw.get();
                 CacheVec<uint32_t, E / 4> c;
 #pragma unroll
                 for (int j = 0; j < E / 4; ++j) {
                     int q = __builtin_amdgcn_cvt_pk_fp8_f32(quotient((float)r.v[4 * j]), quotient((float)r.v[4 * j + 1]), 0, false);
                     c.v[j] = __builtin_amdgcn_cvt_pk_fp8_f32(quotient((float)r.v[4 * j + 2]), quotient((float)r.v[4 * j + 3]), q, true);
                 }
-                *(CacheVec<uint32_t, E / 4> *)(k + (int64_t)(o + i) * p.cache.k_st + lane % LPR * E) = c;
+                if (i < n) *(CacheVec<uint32_t, E / 4> *)(k + (int64_t)(o + i) * p.cache.k_st + lane % LPR * E) = c;
+            };
+            const int first = lane / LPR;
+            float a = 0.f;
+            Row r[kAppendRows] = {};
+            // (a run of a few rows, the usual one of a decoding step, is one vector)
+            const bool few = n <= RPI, fits = n <= kAppendRows * RPI;
+            if (few) {
+                r[0] = row_at(first);
+                a = finite_max(r[0].get(), a);
+            } else {
+                for (int i = first; i < n; i += kAppendRows * RPI) {
+#pragma unroll
+                    for (int j = 0; j < kAppendRows; ++j) r[j] = row_at(i + j * RPI);
+#pragma unroll
+                    for (int j = 0; j < kAppendRows; ++j) {
+                        a = finite_max(r[j].get(), a);
+                        __builtin_amdgcn_sched_barrier(0);   // a row's fp32 values at a time
+                    }
+                }
             }
-            if (grown)
+            rescale(a);
+#pragma unroll
+            for (int j = 0; j < kAppendRows; ++j)
+                if (j == 0 || !few) r[j].settle();
+            with_quotient(now, [&](const auto &quotient) {
+                if (few) {
+                    store(r[0], first, quotient);
+                    return;
+                }
+                for (int i = first; i < n; i += kAppendRows * RPI) {
+                    if (!fits)
+#pragma unroll
+                        for (int j = 0; j < kAppendRows; ++j) r[j] = row_at(i + j * RPI);
+#pragma unroll
+                    for (int j = 0; j < kAppendRows; ++j) {
+                        store(r[j], i + j * RPI, quotient);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
+            });
+            if (grown) {
+                const float shrink = was / now;
                 for (int i = lane / (D / 4); i < o; i += 64 / (D / 4)) {
                     uint32_t *c = (uint32_t *)(k + (int64_t)i * p.cache.k_st + lane % (D / 4) * 4);
                     *c = cache_rescale(*c, shrink);
                 }
+            }
         } else {
             uint8_t *v = p.cache.v + page * p.cache.v_sp + head * p.cache.v_sh;
             constexpr int LPC = D / 2;            // lanes that cover the columns, two each
             const int d = lane % LPC * 2;
-            for (int g = (grown ? 0 : o / 16) + lane / LPC; g < (o + n + 15) / 16; g += 64 / LPC) {
-                uint8_t *c0 = v + (int64_t)d * p.cache.v_sd + g * 16, *c1 = c0 + p.cache.v_sd;
-                CacheVec<uint32_t, 4> a0 = *(CacheVec<uint32_t, 4> *)c0, a1 = *(CacheVec<uint32_t, 4> *)c1;
-                CacheVec<T, 2> r[16];
+            typedef CacheRaw<T, 2> Pair;
+            typedef CacheVec<uint32_t, 4> Codes;
+            // 16 tokens of a page from 16 g on; those outside the run: one of its own, not used
+            Pair r[16] = {};
+            const auto read = [&](int g) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i)      // tokens outside the run: one of its own, not used
-                    r[i] = *(const CacheVec<T, 2> *)(x + min(max(g * 16 + i - o, 0), n - 1) * st + d);
+                for (int i = 0; i < 16; ++i) r[i].load(x + min(max(g * 16 + i - o, 0), n - 1) * st + d);
+            };
+            const int g0 = o / 16, g1 = (o + n + 15) / 16;
+            const bool fits = g1 - g0 == 1;
+            Codes a0, a1;
+            uint8_t *c0 = v + (int64_t)d * p.cache.v_sd + g0 * 16, *c1 = c0 + p.cache.v_sd;
+            float a = 0.f;
+            if (fits) {
+                a0 = *(Codes *)c0, a1 = *(Codes *)c1;
+                read(g0);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int at = g * 16 + 4 * j;
-                    const uint32_t fresh = byte_mask(at, o, o + n), old = byte_mask(at, 0, o);
-                    const auto pack = [&](int c) -> uint32_t {
-                        int q = __builtin_amdgcn_cvt_pk_fp8_f32(quotient((float)r[4 * j].v[c]), quotient((float)r[4 * j + 1].v[c]), 0, false);
-                        return __builtin_amdgcn_cvt_pk_fp8_f32(quotient((float)r[4 * j + 2].v[c]), quotient((float)r[4 * j + 3].v[c]), q, true);
-                    };
-                    if (grown) {
-                        a0.v[j] = (cache_rescale(a0.v[j], shrink) & old) | (a0.v[j] & ~old);
-                        a1.v[j] = (cache_rescale(a1.v[j], shrink) & old) | (a1.v[j] & ~old);
-                    }
-                    a0.v[j] = (pack(0) & fresh) | (a0.v[j] & ~fresh);
-                    a1.v[j] = (pack(1) & fresh) | (a1.v[j] & ~fresh);
+                for (int i = 0; i < 16; ++i) a = finite_max(r[i].get(), a);
+            } else {
+                for (int i = lane / LPR; i < n; i += 4 * RPI) {
+                    Row y[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) y[j] = row_at(i + j * RPI);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) a = finite_max(y[j].get(), a);
                 }
-                *(CacheVec<uint32_t, 4> *)c0 = a0;
-                *(CacheVec<uint32_t, 4> *)c1 = a1;
             }
+            rescale(a);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) r[i].settle();
+            const float shrink = was / now;
+            const bool again = !fits || grown;
+            with_quotient(now, [&](const auto &quotient) {
+                for (int g = (grown ? 0 : g0) + (again ? lane / LPC : 0); g < g1; g += again ? 64 / LPC : 1) {
+                    if (again) {
+                        c0 = v + (int64_t)d * p.cache.v_sd + g * 16, c1 = c0 + p.cache.v_sd;
+                        a0 = *(Codes *)c0, a1 = *(Codes *)c1;
+                        read(g);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int at = g * 16 + 4 * j;
+                        const uint32_t fresh = byte_mask(at, o, o + n), old = byte_mask(at, 0, o);
+                        const auto pack = [&](int c) -> uint32_t {
+                            int q = __builtin_amdgcn_cvt_pk_fp8_f32(quotient((float)r[4 * j].get().v[c]), quotient((float)r[4 * j + 1].get().v[c]), 0, false);
+                            return __builtin_amdgcn_cvt_pk_fp8_f32(quotient((float)r[4 * j + 2].get().v[c]), quotient((float)r[4 * j + 3].get().v[c]), q, true);
+                        };
+                        if (grown) {
+                            a0.v[j] = (cache_rescale(a0.v[j], shrink) & old) | (a0.v[j] & ~old);
+                            a1.v[j] = (cache_rescale(a1.v[j], shrink) & old) | (a1.v[j] & ~old);
+                        }
+                        a0.v[j] = (pack(0) & fresh) | (a0.v[j] & ~fresh);
+                        a1.v[j] = (pack(1) & fresh) | (a1.v[j] & ~fresh);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    *(Codes *)c0 = a0;
+                    *(Codes *)c1 = a1;
+                }
+            });
         }
     }
 }
