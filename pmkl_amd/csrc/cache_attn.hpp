@@ -677,9 +677,11 @@ struct CacheJoin {
     }
 };
 
-// A workgroup for each row block, whose NW waves split its tiles.
+// A workgroup for each row block, whose NW waves split its tiles.  (Waves of a SIMD:
+// fp32 at head_dim 128 spills with two, 16 requests of 1,000 keys 21.1 us, with one
+// 16.2; fp16 spills less, 17.2 and 15.2, but 128 requests 36.6 and 44.8.)
 template <typename T, int D, int NW>
-__global__ __launch_bounds__(NW * 64, D >= 128 ? 2 : 3) void cache_attn_kernel(CacheAttnParams p) {
+__global__ __launch_bounds__(NW * 64, D >= 128 ? (CacheQuery<T>::QT > 1 ? 1 : 2) : 3) void cache_attn_kernel(CacheAttnParams p) {
     __shared__ __attribute__((aligned(16))) CacheJoin<D, NW> join;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     CacheItem it;
@@ -702,10 +704,12 @@ __global__ __launch_bounds__(NW * 64, D >= 128 ? 2 : 3) void cache_attn_kernel(C
     }
 }
 
-// From so many rows on a request is a chunk: where the call has many rows, chunks
-// have a form of their own.
-constexpr int kChunkFrom = 64;
-__device__ __forceinline__ bool cache_is_chunk(const CacheAttnParams &p, const CacheItem &r) { return cache_rows(p, r) >= kChunkFrom; }
+// Where the call has many rows, a request with the rows of a workgroup or more is
+// a chunk and has a form of its own (64 requests of 128 rows 82 us, in the split
+// form 103; of 64 rows 75 and 67).
+constexpr int kChunkBlocks = 1, kChunkWaves = 8;
+constexpr int kChunkRows = kCacheRows * kChunkBlocks * kChunkWaves;
+__device__ __forceinline__ bool cache_is_chunk(const CacheAttnParams &p, const CacheItem &r) { return cache_rows(p, r) >= kChunkRows; }
 
 // The tiles of all row blocks, one after the other (requests, then heads, then
 // blocks), in equal ranges of a wave each, however the requests' lengths differ:
@@ -799,8 +803,17 @@ __device__ __forceinline__ void cache_split(const CacheAttnParams &p, int range,
 
 constexpr int kSplitWaves = 4;   // of a workgroup: they share nothing
 
+// Waves that a SIMD holds of the kernel, whose registers are as many as that leaves:
+// with fewer they spill (head_dim 128 in two terms, 128 requests of 16 k, us: one wave
+// 186 in fp16 and 191 in fp32, two 294 and 340; head_dim 64 in fp16, 64 requests of 4 k:
+// two 17.7, three 22.1; head_dim 32 three 27.0, two 30.2).
 template <typename T, int D>
-__global__ __launch_bounds__(kSplitWaves * 64, D >= 128 ? 2 : 3) void cache_attn_split_kernel(CacheAttnParams p) {
+__host__ __device__ constexpr int cache_split_waves() {
+    return D >= 128 && CacheQuery<T>::PT > 1 ? 1 : D >= 64 ? 2 : 3;
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(kSplitWaves * 64, (cache_split_waves<T, D>())) void cache_attn_split_kernel(CacheAttnParams p) {
     cache_split<T, D>(p, blockIdx.x * kSplitWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), p.ranges);
 }
 
@@ -808,9 +821,9 @@ __global__ __launch_bounds__(kSplitWaves * 64, D >= 128 ? 2 : 3) void cache_attn
 // at PER ranges and takes their blocks one after the other; a row has NW waves,
 // over the rows (a power of two), whose D / 4 lanes have the columns of a part.
 // Parts come from the L2s of other dies, 2 us away: a wave has eight on the way at
-// once, with what they weigh.  Few blocks of many parts: NW 16, PER 8 (64 parts in
-// 4.5 us, by four waves with the largest weight looked up first 14); else a
-// workgroup of four waves for each range.
+// once, with what they weigh.  Blocks of more than 64 parts take NW 16, PER 4, blocks of
+// a few NW 4, PER 1, others NW 8, PER 2 (the attention with each, us: 128 parts 19.9,
+// 28.5, 22.8; 6 parts 36.0, 27.0, 29.5; 25 parts 23.1, 17.7, 18.5 to 22.8, 15.9, 15.4).
 template <typename T, int D, int NW, int PER>
 __global__ __launch_bounds__(NW * 64) void cache_attn_join_kernel(CacheAttnParams p) {
     __shared__ __attribute__((aligned(16))) float share[NW][D];
@@ -897,9 +910,6 @@ __global__ __launch_bounds__(NW * 64) void cache_attn_join_kernel(CacheAttnParam
 // them into the LDS as the operands that the products take: a code is converted
 // once for 128 rows.  In the LDS 16-byte pieces change places within a row, by the
 // row's number, so that the 16 rows that a read takes lie in all banks.
-constexpr int kChunkBlocks = 1, kChunkWaves = 8;
-constexpr int kChunkRows = kCacheRows * kChunkBlocks * kChunkWaves;
-
 template <typename frag, int D>
 struct CacheStage {
     static constexpr int KP = D / 16;                       // 16-code pieces of a key (of a column: 4)
@@ -1013,8 +1023,10 @@ __device__ __forceinline__ void cache_chunk(const CacheAttnParams &p, uint8_t *s
     CacheItem it;
     if (!cache_find(p, i, lane, it, [&](const CacheItem &r) { return blocks(r) * p.kv_heads; })) return;
     const int n = blocks(it);
-    it.head = i / n;
-    const int row0 = __builtin_amdgcn_readfirstlane(i % n * kChunkRows);
+    // The rows that see the most first (a whole prompt of 8,192 tokens 645 us, in
+    // rows' order 970), and for each the heads, so that dies have heads of their own.
+    it.head = i % p.kv_heads;
+    const int row0 = __builtin_amdgcn_readfirstlane((n - 1 - i / p.kv_heads) * kChunkRows);
     it.row0 = row0 + wave * kChunkBlocks * kCacheRows;
     cache_uniform(it);
     const int64_t rows = cache_rows(p, it);
@@ -1111,8 +1123,10 @@ __device__ __forceinline__ void cache_chunk(const CacheAttnParams &p, uint8_t *s
     }
 }
 
+// Two workgroups of a CU; one where three terms of a query of 128 columns would spill
+// (fp32, a prompt of 8,192 tokens: 725 us, with two 924).
 template <typename T, int D>
-__global__ __launch_bounds__(kChunkWaves * 64, kChunkWaves / 2) void cache_attn_chunk_kernel(CacheAttnParams p) {
+__global__ __launch_bounds__(kChunkWaves * 64, kChunkWaves / 4 * (D >= 128 && CacheQuery<T>::QT > 1 ? 1 : 2)) void cache_attn_chunk_kernel(CacheAttnParams p) {
     __shared__ __attribute__((aligned(16))) uint8_t smem[2 * CacheStage<typename CacheQuery<T>::frag, D>::BYTES];
     __shared__ int bad;
     cache_chunk<T, D>(p, smem, &bad, blockIdx.x);

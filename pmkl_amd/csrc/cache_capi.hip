@@ -263,19 +263,26 @@ int run_append(const pmkl_cache_append_args *a, void *stream) {
 typedef void (*cache_attn_fn)(CacheAttnParams);
 constexpr int kAttnWaves = 4;
 constexpr int64_t kChunkRows = pmkl_amd::kChunkRows;
-constexpr int64_t kWholeKeys = 1024;
 
-constexpr int kJoinPer = 8, kJoinWaves = 4;
+// The join's waves of a workgroup and ranges that it looks at.
+struct JoinShape {
+    int waves, per;
+};
+constexpr JoinShape kJoins[3] = {{4, 1}, {8, 2}, {16, 4}};
 
 struct AttnKernels {
-    cache_attn_fn whole, split, chunk, join, join_many;
+    cache_attn_fn whole, split, chunk, joins[3];
+    int split_waves;   // that a SIMD holds of `split`
 };
 
 template <typename T, int D>
 AttnKernels attn_kernels() {
     return {pmkl_amd::cache_attn_kernel<T, D, kAttnWaves>, pmkl_amd::cache_attn_split_kernel<T, D>,
-            pmkl_amd::cache_attn_chunk_kernel<T, D>, pmkl_amd::cache_attn_join_kernel<T, D, kJoinWaves, 1>,
-            pmkl_amd::cache_attn_join_kernel<T, D, 16, kJoinPer>};
+            pmkl_amd::cache_attn_chunk_kernel<T, D>,
+            {pmkl_amd::cache_attn_join_kernel<T, D, kJoins[0].waves, kJoins[0].per>,
+             pmkl_amd::cache_attn_join_kernel<T, D, kJoins[1].waves, kJoins[1].per>,
+             pmkl_amd::cache_attn_join_kernel<T, D, kJoins[2].waves, kJoins[2].per>},
+            pmkl_amd::cache_split_waves<T, D>()};
 }
 template <typename T>
 AttnKernels pick_attn(int64_t D) {
@@ -290,7 +297,7 @@ struct AttnPlan {
     AttnKernels fn;
     bool split;
     int64_t grid, threads, ranges;
-    bool join_many;   // blocks of many parts
+    int join;         // which of kJoins
     int64_t chunks;   // workgroups of the chunks' form, beside the split one; 0: it is not used
     uint64_t parts, workspace;   // bytes: of the split form's parts, in all
     bool empty;
@@ -328,21 +335,35 @@ int plan_attn(const pmkl_cache_attn_args *a, AttnPlan *pl) {
     const int64_t tiles = (a->table_width * a->cache.page_size + pmkl_amd::kCacheTile - 1) / pmkl_amd::kCacheTile +
                           pmkl_amd::kBlockCost;
     pl->threads = kAttnWaves * 64;
-    pl->split = a->table_width * a->cache.page_size > kWholeKeys && pl->grid <= INT32_MAX / tiles;
+    // Chunks have their own form where rows are enough for a workgroup of 128 on every
+    // CU, and by as much more as a row costs less: a workgroup's tiles take their time
+    // however few there are.  us, and in the split form alone: head_dim 128 in bf16,
+    // 16,384 rows of all heads 69, 49; 24,576: 68, 68; 32,768: 69, 84; 65,536: 74, 122; in
+    // fp32 32,768: 99, 132; head_dim 64 at 65,536 71, 73 (fp32 103, 128); head_dim 32 at
+    // 131,072 73, 78.  A call of single tokens has none.
+    const int64_t heads = a->cache.kv_heads, rows = a->tokens * G;
+    const bool many = a->tokens >= 2 * a->batch;
+    if (many && rows * heads * D >= kChunkRows * 256 * 128)
+        pl->chunks = (rows / kChunkRows + std::min(std::min(a->batch, a->tokens), rows / kChunkRows)) * heads;
+    // A table for so few tokens is not worth a second launch, to join: a request of 1,024
+    // keys 13.2 us and 12.5 split, 512 keys 8.6 and 11.7, 2,048 keys 21.6 and 13.3
+    // (head_dim 128); 1,536 keys of head_dim 64 12.6 and 12.1, 1,024 keys 9.0 and 13.8.
+    pl->split = (a->table_width * a->cache.page_size > (D >= 128 ? 1024 : 1536) || pl->chunks) && pl->grid <= INT32_MAX / tiles;
+    if (!pl->split) pl->chunks = 0;
     if (pl->split) {
         const int64_t blocks = pl->grid;
-        // as many waves as the chip's 1,024 SIMDs hold of the kernel
-        pl->ranges = 1024 * (D >= 128 ? 2 : 3);
+        // As many waves as the chip's 1,024 SIMDs hold of the kernel.  But single tokens of
+        // head_dim 128 are bound by loads, and one wave a SIMD has as many on the way as
+        // the memory takes (bf16, 16 requests of 4 k 20.1 us, with two 21.6; 128 of 16 k
+        // 177.6 and 176.8) and leaves half as many parts (4 of 4 k: 18.1 and 20.9); rows of
+        // a chunk are bound by arithmetic (256 tokens: 122 and 102).
+        pl->ranges = 1024 * (D >= 128 && !many ? 1 : pl->fn.split_waves);
         pl->grid = pl->ranges / pmkl_amd::kSplitWaves;
         pl->threads = pmkl_amd::kSplitWaves * 64;
         pl->parts = (uint64_t)2 * pl->ranges * pmkl_amd::kCacheRows * (D + 2) * sizeof(float);
         pl->workspace = pl->parts + pl->ranges * sizeof(pmkl_amd::CacheUnfinished);
         // at most so many blocks have parts, and all of them together few more parts than ranges
-        pl->join_many = blocks * 24 < pl->ranges;
-        // enough rows for a workgroup of 128 on every CU: chunks in their own form
-        const int64_t heads = a->cache.kv_heads, rows = a->tokens * G;
-        if (rows * heads >= kChunkRows * 256)
-            pl->chunks = (rows / kChunkRows + std::min(std::min(a->batch, a->tokens), rows / pmkl_amd::kChunkFrom)) * heads;
+        pl->join = blocks * 64 < pl->ranges ? 2 : blocks * 8 < pl->ranges ? 1 : 0;
     }
     PMKL_REQUIRE(pl->grid * pl->threads < (int64_t(1) << 32) && pl->chunks * pmkl_amd::kChunkWaves * 64 < (int64_t(1) << 32),
                  PMKL_EINVAL, "grid too large (%lld workgroups)", (long long)std::max(pl->grid, pl->chunks));
@@ -402,10 +423,9 @@ int run_attn(const pmkl_cache_attn_args *a, void *stream) {
         hipLaunchKernelGGL(pl.fn.chunk, dim3((unsigned)pl.chunks), dim3(pmkl_amd::kChunkWaves * 64), 0, (hipStream_t)stream, p);
         PMKL_TRY(launched("cache_attn_chunk"));
     }
-    if (pl.join_many)
-        hipLaunchKernelGGL(pl.fn.join_many, dim3((unsigned)pl.ranges / kJoinPer), dim3(1024), 0, (hipStream_t)stream, p);
-    else
-        hipLaunchKernelGGL(pl.fn.join, dim3((unsigned)pl.ranges), dim3(kJoinWaves * 64), 0, (hipStream_t)stream, p);
+    const JoinShape join = kJoins[pl.join];
+    hipLaunchKernelGGL(pl.fn.joins[pl.join], dim3((unsigned)(pl.ranges / join.per)), dim3((unsigned)join.waves * 64), 0,
+                       (hipStream_t)stream, p);
     return launched("cache_attn_join");
 }
 
@@ -448,9 +468,8 @@ const char *pmkl_cache_attn_kernel_name(const pmkl_cache_attn_args *a) {
         n += snprintf(name + n, sizeof(name) - n, ", cache_attn_chunk_kernel<%s, %lld> grid %lld x %d", dt, D,
                       (long long)pl.chunks, pmkl_amd::kChunkWaves * 64);
     if (pl.split)
-        snprintf(name + n, sizeof(name) - n, ", cache_attn_join_kernel<%s, %lld, %d, %d> grid %lld x %d", dt, D,
-                 pl.join_many ? 16 : kJoinWaves, pl.join_many ? kJoinPer : 1, (long long)(pl.join_many ? pl.ranges / kJoinPer : pl.ranges),
-                 pl.join_many ? 1024 : kJoinWaves * 64);
+        snprintf(name + n, sizeof(name) - n, ", cache_attn_join_kernel<%s, %lld, %d, %d> grid %lld x %d", dt, D, kJoins[pl.join].waves,
+                 kJoins[pl.join].per, (long long)(pl.ranges / kJoins[pl.join].per), kJoins[pl.join].waves * 64);
     return name;
 }
 

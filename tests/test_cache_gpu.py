@@ -190,7 +190,8 @@ def test_chunks(device, dtype, dim, page, kv_heads, group, causal):
     cache.v_scale[cache.table[2, 0]] *= 2.0 ** 30 if dtype != "fp16" else 2.0 ** 4
     cache.v_scale[cache.table[5, -(-65 // page) - 1]] *= 2.0 ** -30
     cache.refresh()
-    q = _q(sum(new) + 10, kv_heads * group, dim, dtype, seed=dim)
+    # rows of no request make it a call of many rows
+    q = _q(max(sum(new) + 10, 2 ** 23 // (kv_heads * group * dim) + 1), kv_heads * group, dim, dtype, seed=dim)
     assert _form(cache, q) == "chunk"
     out, m, l = _attend(cache, q, new, causal=causal, label=f"{dtype} {dim}")
     if causal:
@@ -200,7 +201,7 @@ def test_chunks(device, dtype, dim, page, kv_heads, group, causal):
 
 def test_forms(device):
     """The sizes of these tests reach every form."""
-    for lengths, tokens, heads, form in (([1000], 1, 4, "whole"), ([1100], 1, 4, "split"), ([1100], 2000, 32, "chunk")):
+    for lengths, tokens, heads, form in (([1500], 1, 4, "whole"), ([1600], 1, 4, "split"), ([300], 2100, 32, "chunk")):
         assert _form(Cache(lengths, 2, 16, 64, seed=1, width_more=0), _q(tokens, heads, 64, "bf16", 1)) == form
 
 
