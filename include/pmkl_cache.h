@@ -162,7 +162,7 @@ typedef struct pmkl_cache_attn_args {
  * the cache holds there); a row that sees none has o = 0, m = -inf, l = 0.  NaN in a
  * hidden token reaches nothing.  Rows of no request are not written.  query_start must
  * not decrease and is clamped to 0 .. tokens; where it decreases, what the call's rows
- * hold is unspecified (nothing else is touched).
+ * hold is unspecified, and some may not be written (nothing else is touched).
  * The same call gives the same bits every time. */
 int pmkl_cache_attn_fwd(const pmkl_cache_attn_args *args, void *stream);
 

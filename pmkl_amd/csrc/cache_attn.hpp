@@ -197,6 +197,12 @@ __device__ __forceinline__ void cache_uniform(CacheItem &it) {
     it.keys = __builtin_amdgcn_readfirstlane(it.keys);
 }
 
+// Whether request b starts behind its end.  Past such a one the sums below would not
+// be bounded by what the host has checked: nothing is looked for there.
+__device__ __forceinline__ bool cache_falls(const CacheAttnParams &p, int b) {
+    return b < p.batch && p.query_start[b + 1] < p.query_start[b];
+}
+
 // Requests in order have weight(request) units each (fewer than 2^31 in all:
 // checked); finds the one with unit i, and i counted from its first.  Every wave
 // sums by itself, 64 requests at a time.  False past the last unit.
@@ -204,6 +210,7 @@ template <typename Weight>
 __device__ __forceinline__ bool cache_find(const CacheAttnParams &p, int &i, int lane, CacheItem &it, Weight weight) {
     for (int base = 0; base < p.batch; base += 64) {
         const int b = base + lane;
+        if (__builtin_amdgcn_ballot_w64(cache_falls(p, b))) return false;
         const int own = b < p.batch ? weight(cache_request(p, b)) : 0;
         const int end = wave_scan(own);
         const uint64_t mask = __builtin_amdgcn_ballot_w64(i < end);
@@ -217,6 +224,7 @@ __device__ __forceinline__ bool cache_find(const CacheAttnParams &p, int &i, int
     }
     return false;
 }
+
 // A head's pages.  Strides between pages are below 2^31 (checked): a page's place
 // is one multiply-add.
 struct CacheHead {
@@ -739,9 +747,13 @@ __device__ __forceinline__ void cache_split(const CacheAttnParams &p, int range,
     // of the first 64 requests, and of all
     const int own = weight(lane), sums = wave_scan(own), first = __builtin_amdgcn_readlane(sums, 63);
     int rest = 0;
-    for (int b = 64 + lane; b < p.batch; b += 64) rest += weight(b);
+    bool falls = cache_falls(p, lane);
+    for (int b = 64 + lane; b < p.batch; b += 64) {
+        rest += weight(b);
+        falls = falls || cache_falls(p, b);
+    }
     if (p.batch > 64) rest = __builtin_amdgcn_readlane(wave_scan(rest), 63);
-    const int total = first + rest;
+    const int total = __builtin_amdgcn_ballot_w64(falls) ? 0 : first + rest;
     ranges = min(ranges, total);          // none is empty
     const auto begin_of = [&](int r) { return (int)((int64_t)r * total / ranges); };
     const int lo = range < ranges ? begin_of(range) : 0, hi = range < ranges ? begin_of(range + 1) : 0;

@@ -315,6 +315,37 @@ def test_starts_past_the_rows_are_clamped(device):
         assert (out == 7).all() == (starts == [0, 0, 0, 0])
 
 
+@pytest.mark.parametrize("width_more,tokens", [(0, 0), (200, 0), (0, 2200)])
+def test_starts_that_fall(device, width_more, tokens):
+    """query_start must not decrease.  Where it does nothing but the call's rows is written, in every form, however often
+    requests name the same rows."""
+    import torch
+
+    import pmkl_amd
+
+    cache = Cache([40] * 70, 1, 16, 64, seed=21, width_more=width_more)
+    tokens = tokens or 70
+    q = _q(tokens, 32, 64, "bf16", seed=21)
+    big = torch.full((tokens + 2, 32, 64), 7.0, dtype=q.dtype, device="cuda:0")
+    for starts in ([tokens] + [0] * 70, [0, tokens] * 35 + [0], list(range(71))[::-1], [0] * 66 + [2**31 - 1, -2**31] * 2 + [0]):
+        pmkl_amd.cache_attn_fwd(q, **cache.tensors, block_table=_int32(cache.table), seq_lens=_int32([40] * 70),
+                                query_start=_int32(starts), out=big[1:-1])
+    torch.cuda.synchronize()
+    assert (big[0] == 7).all() and (big[-1] == 7).all()
+
+
+@pytest.mark.parametrize("longest", [700, 2000])
+def test_many_requests(device, longest):
+    """More requests than a wave has lanes, some of no tokens, their lengths far apart, in the whole and the split form."""
+    rng = np.random.default_rng(22)
+    lengths = [int(longest ** rng.uniform()) for _ in range(149)] + [longest]
+    new = [int(rng.choice([0, 1, 1, 1, min(n, 5)])) for n in lengths]
+    cache = Cache(lengths, 2, 16, 64, seed=22, width_more=0)
+    q = _q(sum(new), 4, 64, "fp16", seed=22)
+    assert _form(cache, q) == ("whole" if longest < 1000 else "split")
+    _attend(cache, q, new, label=f"{longest}")
+
+
 def test_offsets_past_32_bits(device):
     """Pages 300 MiB apart: the last ones lie past 4 GiB; and a token stride of 1 MiB within a page."""
     import torch
