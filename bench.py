@@ -61,9 +61,9 @@ def parse_args():
                     help="also time torch's scaled_dot_product_attention on the same tensors (reference point; "
                          "restricted to its flash / memory-efficient backends: the math fallback runs "
                          "transposed bf16 batched products)")
-    ap.add_argument("--op", default="fwd", choices=["fwd", "bwd", "softmax"],
+    ap.add_argument("--op", default="fwd", choices=["fwd", "bwd", "softmax", "cache"],
                     help="fwd: the headline forward (default); bwd: the backward (pmkl_attn_bwd), "
-                         "its own JSON line")
+                         "its own JSON line; softmax: the row softmax; cache: a serving step over the 8-bit cache")
     ap.add_argument("--calibrate-copy", action="store_true",
                     help="run only a plain 512 MiB device copy (torch copy kernel) so that rocprofv3 "
                          "FETCH_SIZE / WRITE_SIZE can be scaled against a known byte count")
@@ -472,6 +472,91 @@ def bench_softmax(args):
     print(json.dumps(line), flush=True)
 
 
+CACHE_STEP = dict(batch=64, heads=32, kv_heads=8, head_dim=128, page=16, longest=4096)
+
+
+def bench_cache(args):
+    """One layer's serving step over the 8-bit cache: 64 requests of 128 to 4,096
+    cached tokens (log-uniform) get a token each - its block table entry and slot
+    (pmkl_cache_slots), its key and value into the cache (pmkl_cache_append) and its
+    attention over all of the request (pmkl_cache_attn_fwd), bf16, 32 query and 8 key
+    heads of 128, pages of 16.  Timed as the three calls (value) and as replays of a HIP
+    graph of them.  Bytes: the cached codes and scales, read once."""
+    import numpy as np
+    import torch
+
+    import pmkl_amd
+
+    c = CACHE_STEP
+    B, H, Hk, D, page, longest = (c[x] for x in ("batch", "heads", "kv_heads", "head_dim", "page", "longest"))
+    dev = torch.device("cuda:0")
+    rng = np.random.Generator(np.random.PCG64(1007))
+    cached = np.exp(rng.uniform(np.log(128), np.log(longest), B)).astype(np.int32)
+    cached[0] = longest
+    held = -(-cached // page)
+    width, pages = int(held.max()) + 1, int(held.sum()) + B
+    order = rng.permutation(pages).astype(np.int32)
+    table = np.full((B, width), -1, np.int32)
+    table[np.arange(width) < held[:, None]] = order[:held.sum()]
+    g = torch.Generator(device=dev).manual_seed(1007)
+    caches = {}
+    for name, shape in (("k_cache", (pages, Hk, page, D)), ("v_cache", (pages, Hk, D, page))):
+        x = torch.randn(shape, generator=g, device=dev).mul_(100).clamp_(-448, 448)
+        caches[name] = x.to(torch.float8_e4m3fn)
+    for name in ("k_scale", "v_scale"):
+        caches[name] = torch.full((pages, Hk), 2.0 ** -6, device=dev)
+    packed = torch.randn((B, H + 2 * Hk, D), generator=g, device=dev).to(torch.bfloat16)
+    q, k, v = packed.split([H, Hk, Hk], 1)
+    lens, table, free = (torch.from_numpy(x).to(dev) for x in (cached, table, order[held.sum():].copy()))
+    new, head = torch.ones(B, dtype=torch.int32, device=dev), torch.zeros(1, dtype=torch.int32, device=dev)
+
+    def step():
+        seq_lens, start, slots, _ = pmkl_amd.cache_slots(lens, new, table, free, head, page, B)
+        pmkl_amd.cache_append(k, v, slots, **caches)
+        return pmkl_amd.cache_attn_fwd(q, **caches, block_table=table, seq_lens=seq_lens, query_start=start)
+
+    def timed(f):
+        t_w = time.perf_counter()
+        while time.perf_counter() - t_w < args.warmup_seconds:
+            for _ in range(max(args.warmup, 1)):
+                f()
+            torch.cuda.synchronize()
+        ev0, ev1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        ev0.record()
+        for _ in range(args.steps):
+            f()
+        ev1.record()
+        torch.cuda.synchronize()
+        return ev0.elapsed_time(ev1) / args.steps
+
+    ms = timed(step)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    graph_ms = timed(graph.replay)
+    read = int(cached.sum() + B) * Hk * D * 2 + int(held.sum()) * Hk * 8
+    achieved = read / (ms / 1e3) / 1e9
+    print(json.dumps({
+        "metric": f"serving step tokens/s on 1 MI355X, bf16 over an 8-bit cache, B{B} H{H}/{Hk} D{D}",
+        "value": round(B / (ms / 1e3), 1),
+        "unit": "tokens/s",
+        "n_gpus": 1,
+        "steps": args.steps,
+        "warmup": args.warmup,
+        "ms_per_step": round(ms, 4),
+        "higher_is_better": True,
+        "scaling": "weak",
+        "vs_baseline": None,
+        "dtype": "bf16",
+        "data": "synthetic: N(0,1) and seeded PCG64 lengths (seed 1007)",
+        "config": {"workload": "cache_slots, cache_append and cache_attn_fwd of one layer",
+                   "global_batch": B, "cached_tokens": int(cached.sum()), "page_size": page, "bytes_read_per_step": read},
+        "roofline": {"bound": "hbm", "achieved": round(achieved, 1), "peak": PEAK_HBM_GBS, "unit": "GB/s",
+                     "frac": round(achieved / PEAK_HBM_GBS, 4)},
+        "graph": {"what": "replays of a HIP graph of the same calls", "ms_per_step": round(graph_ms, 4)},
+    }), flush=True)
+
+
 def torch_sdpa_reference(q, k, v, flops, steps):
     """Reference point, timed after the timed region: torch's own
     scaled_dot_product_attention (causal, default scale 1/sqrt(D)) on the
@@ -513,6 +598,9 @@ def main():
         return
     if args.op == "softmax":
         bench_softmax(args)
+        return
+    if args.op == "cache":
+        bench_cache(args)
         return
 
     import torch
