@@ -685,9 +685,11 @@ struct CacheJoin {
     }
 };
 
-// A workgroup for each row block, whose NW waves split its tiles.  (Waves of a SIMD:
-// fp32 at head_dim 128 spills with two, 16 requests of 1,000 keys 21.1 us, with one
-// 16.2; fp16 spills less, 17.2 and 15.2, but 128 requests 36.6 and 44.8.)
+// A workgroup for each row block, whose NW waves split its tiles.  One request of 128
+// keys, fp32, 4 heads of 64: 5.3 us, of which a launch is 2.5; the lengths, the table, the
+// tiles and the join come one after the other.
+// Waves of a SIMD: fp32 at head_dim 128 spills with two, 16 requests of 1,000 keys 21.1
+// us, with one 16.2; fp16 spills less, 17.2 and 15.2, but 128 requests 36.6 and 44.8.
 template <typename T, int D, int NW>
 __global__ __launch_bounds__(NW * 64, D >= 128 ? (CacheQuery<T>::QT > 1 ? 1 : 2) : 3) void cache_attn_kernel(CacheAttnParams p) {
     __shared__ __attribute__((aligned(16))) CacheJoin<D, NW> join;
@@ -727,6 +729,10 @@ __device__ __forceinline__ bool cache_is_chunk(const CacheAttnParams &p, const C
 // cache_attn_join_kernel adds up: part 2 w of range w is the one that starts the
 // range, 2 w + 1 one that starts behind it.  `unfinished` tells the join of the
 // block whose first tile is in range w and whose last is not.
+// Bound by the cache's bytes where they are many: 128 requests of 512 to 16,384
+// tokens, 32 heads over 8 of 128, 1.05 GB in 173 us, 6.1 TB/s; by latency where they
+// are few: of the 14 us for 4 of 4,096 (34 MB) some 2.5 go into the lengths and the
+// range's place, 2 into the first tile's loads, 1 into each tile's arithmetic.
 struct CacheUnfinished {
     int rows;         // of the block, 0: there is none
     int q0, head, row0;
@@ -917,11 +923,13 @@ __global__ __launch_bounds__(NW * 64) void cache_attn_join_kernel(CacheAttnParam
     }
 }
 
-// Chunks of prompts: a workgroup has 128 rows, 32 a wave, and all their tiles.  Its
+// Chunks of prompts: a workgroup has 128 rows, 16 a wave, and all their tiles.  Its
 // waves load a tile's codes together, while they work on the one before, and put
 // them into the LDS as the operands that the products take: a code is converted
 // once for 128 rows.  In the LDS 16-byte pieces change places within a row, by the
-// row's number, so that the 16 rows that a read takes lie in all banks.
+// row's number, so that the 16 rows that a read takes lie in all banks.  Bound by
+// what goes beside the products (weights, conversions, LDS reads): 4 chunks of 512 tokens
+// over 4,096, bf16, 32 heads over 8 of 128, 129 GFLOP in 186 us, 690 TFLOP/s.
 template <typename frag, int D>
 struct CacheStage {
     static constexpr int KP = D / 16;                       // 16-code pieces of a key (of a column: 4)
