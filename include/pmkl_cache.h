@@ -120,7 +120,7 @@ typedef struct pmkl_cache_append_args {
  * down to the type's subnormals.  Everything behind the run is left as it was.
  * A slot outside 0 .. pages * page_size - 1 is skipped.  A page may take one run a
  * call: where two runs name the same page, its codes and scales of this call are
- * unspecified (other pages are not touched). */
+ * unspecified (other pages are not touched).  k and v must not overlap the cache. */
 int pmkl_cache_append(const pmkl_cache_append_args *args, void *stream);
 
 /* Arguments of pmkl_cache_attn_fwd. */
@@ -163,6 +163,7 @@ typedef struct pmkl_cache_attn_args {
  * hidden token reaches nothing.  Rows of no request are not written.  query_start must
  * not decrease and is clamped to 0 .. tokens; where it decreases, what the call's rows
  * hold is unspecified, and some may not be written (nothing else is touched).
+ * o, m, l and the workspace must overlap nothing that the call reads.
  * The same call gives the same bits every time. */
 int pmkl_cache_attn_fwd(const pmkl_cache_attn_args *args, void *stream);
 

@@ -267,7 +267,7 @@ def cache_slots(cached_lens, new_lens, block_table, free_pages, free_head, page_
     num_tokens is the sum of new_lens, or more.  Where the list or a table row is
     too short, the tokens concerned have slot -1 (pmkl_cache.h says more); the
     returned free_head is then past F in the first case.  On torch's current stream;
-    nothing is synchronised.
+    nothing is synchronised.  The four tensors share one allocation.
     """
     from . import pmkl_pytorch_ext
 
@@ -302,8 +302,9 @@ def cache_attn_fwd(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens,
     cache_append, block_table int32 [B, W].  is_causal: a token sees itself and what
     lies before it, else all of its request.  scale: 1/sqrt(head_dim) by default.
     Returns (out, out_m, out_l): out in q's dtype, the row max and row sum [N, heads] in
-    float32; given buffers are written and returned.  A row that sees no token has
-    out 0, out_m -inf and out_l 0; rows of no request are not written.  On torch's
+    float32; given buffers are written and returned, the others share one allocation.  A
+    row that sees no token has out 0, out_m -inf and out_l 0; rows of no request are not
+    written.  On torch's
     current stream, with workspace from its allocator.  No backward.
     """
     from . import pmkl_pytorch_ext

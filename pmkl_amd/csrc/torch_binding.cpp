@@ -459,6 +459,34 @@ pmkl_kv_cache cache_of(const char *op, const at::Tensor &like, const at::Tensor 
     return c;
 }
 
+// Results of one call in one allocation: each is a tensor of its own on the shared
+// storage.  (An at::empty each would be a tenth of the smallest calls' time.)
+class Results {
+  public:
+    explicit Results(const at::Tensor &like) : like_(like) {}
+    // where a contiguous tensor begins in the allocation
+    int64_t add(int64_t elements, at::ScalarType type) {
+        const int64_t at = bytes_;
+        bytes_ += (elements * (int64_t)c10::elementSize(type) + 15) / 16 * 16;
+        return at;
+    }
+    void allocate() {
+        all_ = at::empty({bytes_}, like_.options().dtype(at::kByte).memory_format(at::MemoryFormat::Contiguous));
+    }
+    at::Tensor get(int64_t at, at::IntArrayRef sizes, at::ScalarType type) const {
+        auto t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all_.storage()), all_.key_set(),
+                                                          c10::scalarTypeToTypeMeta(type));
+        t.unsafeGetTensorImpl()->set_storage_offset(at / (int64_t)c10::elementSize(type));
+        t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+        return t;
+    }
+
+  private:
+    const at::Tensor &like_;
+    at::Tensor all_;
+    int64_t bytes_ = 0;
+};
+
 void *current_stream(const at::Tensor &t) {
     return (void *)c10::hip::getCurrentHIPStream(t.device().index()).stream();
 }
@@ -486,10 +514,14 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> cache_slots(const at:
                 ": cached_lens, new_lens and free_pages must be contiguous");
     TORCH_CHECK(block_table.numel() == 0 || block_table.size(1) == 1 || block_table.stride(1) == 1, op, ": rows of block_table must be contiguous");
     TORCH_CHECK(num_tokens >= 0, op, ": num_tokens must not be negative");
+    TORCH_CHECK(num_tokens <= INT32_MAX, op, ": num_tokens ", num_tokens, " is past 2^31 - 1");
     c10::OptionalDeviceGuard guard(cached_lens.device());
-    const auto ints = cached_lens.options();
-    auto seq_lens = at::empty({B}, ints), query_start = at::empty({B + 1}, ints), head = at::empty({1}, ints);
-    auto slots = at::empty({num_tokens}, ints.dtype(at::kLong));
+    Results results(cached_lens);
+    const int64_t slots_at = results.add(num_tokens, at::kLong), lens_at = results.add(B, at::kInt),
+                  start_at = results.add(B + 1, at::kInt), head_at = results.add(1, at::kInt);
+    results.allocate();
+    auto seq_lens = results.get(lens_at, {B}, at::kInt), query_start = results.get(start_at, {B + 1}, at::kInt);
+    auto head = results.get(head_at, {1}, at::kInt), slots = results.get(slots_at, {num_tokens}, at::kLong);
     pmkl_cache_slots_args a;
     std::memset(&a, 0, sizeof(a));
     a.cached_lens = static_cast<const int32_t *>(cached_lens.data_ptr());
@@ -568,16 +600,20 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> cache_attn_fwd(
                 ": seq_lens and query_start must be contiguous");
     TORCH_CHECK(block_table.numel() == 0 || block_table.size(1) == 1 || block_table.stride(1) == 1, op, ": rows of block_table must be contiguous");
     TORCH_CHECK(!scale.has_value() || *scale > 0, op, ": scale must be positive");
-    const auto result = [&](const char *name, const std::optional<at::Tensor> &given, at::IntArrayRef sizes,
+    Results results(q);
+    const int64_t out_at = out ? 0 : results.add(N * H * D, q.scalar_type()), m_at = out_m ? 0 : results.add(N * H, at::kFloat),
+                  l_at = out_l ? 0 : results.add(N * H, at::kFloat);
+    const auto result = [&](const char *name, const std::optional<at::Tensor> &given, int64_t at, at::IntArrayRef sizes,
                             at::ScalarType type) {
-        if (!given.has_value()) return at::empty(sizes, q.options().dtype(type).memory_format(at::MemoryFormat::Contiguous));
+        if (!given.has_value()) return results.get(at, sizes, type);
         check_on(op, name, *given, q, type, (int64_t)sizes.size());
         TORCH_CHECK(given->sizes() == sizes, op, ": ", name, " must be ", sizes, ", got ", given->sizes());
         return *given;
     };
     c10::OptionalDeviceGuard guard(q.device());
-    auto o = result("out", out, {N, H, D}, q.scalar_type());
-    auto m = result("out_m", out_m, {N, H}, at::kFloat), l = result("out_l", out_l, {N, H}, at::kFloat);
+    results.allocate();
+    auto o = result("out", out, out_at, {N, H, D}, q.scalar_type());
+    auto m = result("out_m", out_m, m_at, {N, H}, at::kFloat), l = result("out_l", out_l, l_at, {N, H}, at::kFloat);
     TORCH_CHECK(o.numel() == 0 || (o.stride(2) == 1 && !is_expanded(o)), op,
                 ": out must have a contiguous head_dim and not be expanded");
     TORCH_CHECK(m.is_contiguous() && l.is_contiguous(), op, ": out_m and out_l must be contiguous");

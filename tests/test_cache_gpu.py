@@ -299,6 +299,40 @@ def test_strides_and_given_buffers(device):
     _attend(cache, turned, new, label="turned")
 
 
+def test_results_of_one_allocation(device):
+    """Results that are not given lie in one allocation, apart from each other; each is an ordinary tensor that outlives
+    the others, also in inference mode and without tokens."""
+    import torch
+
+    import pmkl_amd
+
+    cache = Cache([50, 33], 2, 16, 32, seed=23)
+    q = _q(5, 2, 32, "fp16", seed=23)
+    given = torch.full((5, 2), 7.0, device="cuda:0")
+    with torch.inference_mode():
+        a = _attend(cache, q, [3, 2], out_m=given, label="inference")
+    b = _attend(cache, q, [3, 2], label="all")
+    assert a[1] is given or a[1].data_ptr() == given.data_ptr()
+    for x, y in zip(a, b):
+        assert x.is_contiguous() and y.is_contiguous() and (x == y).all()
+    spans = sorted((x.data_ptr(), x.data_ptr() + x.numel() * x.element_size()) for x in b)
+    assert all(e <= s for (_, e), (s, _) in zip(spans, spans[1:]))
+    m = b[1]
+    want = m.clone()
+    b[0].add_(1), b[2].zero_()
+    del b
+    junk = [torch.full((4096,), 3.0, device="cuda:0") for _ in range(8)]
+    assert (m == want).all() and m.requires_grad is False and len(junk) == 8
+    (m.clone().requires_grad_(True) * 2).sum().backward()
+    none = pmkl_amd.cache_attn_fwd(q[:0], **cache.tensors, block_table=_int32(cache.table), seq_lens=_int32([50, 33]),
+                                   query_start=_int32([0, 0, 0]))
+    assert [tuple(x.shape) for x in none] == [(0, 2, 32), (0, 2), (0, 2)]
+    lens, start, slots, head = pmkl_amd.cache_slots(_int32([0]), _int32([0]), _int32([[-1]]), _int32([0]), _int32([5]), 16, 0)
+    assert lens.tolist() == [0] and start.tolist() == [0, 0] and slots.shape == (0,) and head.tolist() == [5]
+    with pytest.raises(RuntimeError, match="2\\^31"):
+        pmkl_amd.cache_slots(_int32([0]), _int32([0]), _int32([[-1]]), _int32([0]), _int32([5]), 16, 2 ** 61)
+
+
 def test_starts_past_the_rows_are_clamped(device):
     import torch
 
