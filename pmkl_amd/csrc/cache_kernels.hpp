@@ -273,8 +273,11 @@ __global__ __launch_bounds__(kCacheThreads, 4) void cache_append_kernel(AppendPa
         const int64_t s0 = __shfl(slot, leader);
         const int o = (int)(s0 & (ps - 1));
         const int64_t page = s0 >> log2_page;
-        int n = 0;                                // tokens of the run
-        while (true) {
+        // tokens of the run: of these 64, and behind them
+        const int place = lane - leader;
+        const uint64_t others = ~__builtin_amdgcn_ballot_w64(place >= 0 && place < ps - o && slot == s0 + place) >> leader;
+        int n = others ? __builtin_ctzll(others) : 64 - leader;
+        while (leader + n >= 64) {
             const int i = n + lane;
             const bool in = i < ps - o && t0 + i < p.tokens && p.slots[t0 + i] == s0 + i;
             const uint64_t mask = __builtin_amdgcn_ballot_w64(in);
@@ -287,14 +290,15 @@ __global__ __launch_bounds__(kCacheThreads, 4) void cache_append_kernel(AppendPa
 
         const float *scale = which ? p.cache.v_scale + page * (p.cache.vs_sp / 4) + head * p.cache.vs_sh
                                    : p.cache.k_scale + page * (p.cache.ks_sp / 4) + head * p.cache.ks_sh;
-        const float was = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(*scale)));
+        const float held = *scale;                // on the way with the rows
         const int64_t st = which ? p.v_st : p.k_st;
         const T *x = which ? (const T *)p.v + t0 * p.v_st + head * p.v_sh : (const T *)p.k + t0 * p.k_st + head * p.k_sh;
         // The new scale, and what it is of.
-        float now = 0.f;
+        float was = 0.f, now = 0.f;
         bool grown = false;
         const auto rescale = [&](float a) {
             const float need = cache_scale_for(__uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(wave_max(a)))));
+            was = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(held)));
             const bool kept = o > 0 && was > 0.f && was < INFINITY;
             now = kept ? fmaxf(was, need) : need;
             grown = kept && now != was;
