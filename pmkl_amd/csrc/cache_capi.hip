@@ -249,10 +249,11 @@ int run_append(const pmkl_cache_append_args *a, void *stream) {
     // Of 64 tokens between 64 runs (decoding) and 1 (a prompt in large pages)
     // begin; each is 2 H wave items.  About 8,192 waves in all keep the card
     // busy; more, where a window of a prompt needs them for a page each, and no
-    // more than the items of 64 runs.
+    // more than the items of 64 runs.  In large pages four waves may share an item.
     const int64_t windows = (a->tokens + 63) / 64, waves = pmkl_amd::kCacheThreads / 64;
     const int64_t runs = std::min<int64_t>(64, a->tokens), pages = std::min<int64_t>(runs, 64 / a->cache.page_size + 1);
-    const int64_t y = std::max<int64_t>({1, std::min(runs * 2 * H, 8192 / windows) / waves, pages * 2 * H / waves});
+    const int64_t per = a->cache.page_size >= 64 ? 1 : waves;   // items of a workgroup
+    const int64_t y = std::max<int64_t>({1, std::min(runs * 2 * H / per, 8192 / waves / windows), pages * 2 * H / per});
     const append_fn fn = a->dtype == PMKL_DTYPE_F32 ? pick_append<float>(D)
                          : a->dtype == PMKL_DTYPE_F16 ? pick_append<_Float16>(D) : pick_append<__bf16>(D);
     PMKL_REQUIRE(windows * y * pmkl_amd::kCacheThreads < (int64_t(1) << 32), PMKL_EINVAL, "grid too large");

@@ -245,13 +245,22 @@ __device__ __forceinline__ uint32_t byte_mask(int at, int from, int to) {
 // vector, with the codes around the run read first.  Bound by latency: a decoding
 // step of 256 requests, bf16, 8 heads of 128, 7.4 us (slots, then rows, scales and codes,
 // then stores); 4 prompts of 2,048 tokens, 51 MB, 16.8 us, 3.0 TB/s.
+// In pages of 64 tokens and more a wave would read and write for long: where no more
+// than three runs begin among the 64 tokens, a workgroup's waves take a (run, head,
+// keys or values) together, a share of its rows each, in pages of 64 only while the
+// call has few items (together and by a wave each, us: 8 prompts of 1,000 tokens, 8 heads
+// of 128, pages of 256 25.2, 40.7; 2 of 500 in pages of 128 7.4, 15.8; 24 requests of 1 to 128
+// tokens, pages of 64 6.4, 6.9; but 16 of 64 tokens, 16 heads, pages of 64 7.5, 6.2; 64 of 20
+// 9.7, 6.9).
 constexpr int kAppendRows = 8;   // vectors of a lane that are kept
 
 template <typename T, int D>
 __global__ __launch_bounds__(kCacheThreads, 4) void cache_append_kernel(AppendParams p) {
     constexpr int E = 16 / (int)sizeof(T);      // elements of a vector
     constexpr int LPR = D / E;                    // lanes of a row
-    const int lane = threadIdx.x & 63;
+    constexpr int NW = kCacheThreads / 64;
+    __shared__ float largest[2][NW];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int log2_page = p.cache.log2_page, ps = 1 << log2_page;
     const int64_t limit = (int64_t)p.cache.pages << log2_page;
     const int64_t w0 = (int64_t)blockIdx.x * 64;
@@ -265,8 +274,10 @@ __global__ __launch_bounds__(kCacheThreads, 4) void cache_append_kernel(AppendPa
     const int rank = __builtin_popcountll(leaders & ((1ull << lane) - 1));
     const int items = __builtin_popcountll(leaders) * p.kv_heads * 2;
 
-    const int stride = gridDim.y * (kCacheThreads / 64);
-    for (int item = blockIdx.y * (kCacheThreads / 64) + (threadIdx.x >> 6); item < items; item += stride) {
+    const bool together = ps >= 64 && __builtin_popcountll(leaders) <= 3 && (ps > 64 || (int64_t)items * gridDim.x <= 640);
+    const int sub = together ? wave : 0, of = together ? NW : 1;   // the wave's share
+    int turn = 0;
+    for (int item = together ? blockIdx.y : blockIdx.y * NW + wave; item < items; item += gridDim.y * (NW / of)) {
         const int which = item & 1, head = (item >> 1) % p.kv_heads, run = (item >> 1) / p.kv_heads;
         const int leader = __builtin_ctzll(__builtin_amdgcn_ballot_w64(leads && rank == run));
         const int64_t t0 = w0 + leader;
@@ -297,12 +308,20 @@ __global__ __launch_bounds__(kCacheThreads, 4) void cache_append_kernel(AppendPa
         float was = 0.f, now = 0.f;
         bool grown = false;
         const auto rescale = [&](float a) {
-            const float need = cache_scale_for(__uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(wave_max(a)))));
+            a = wave_max(a);
             was = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(held)));
+            if (together) {
+                if (lane == 0) largest[turn][wave] = a;
+                __syncthreads();                  // (and every wave has the old scale)
+#pragma unroll
+                for (int w = 0; w < NW; ++w) a = fmaxf(a, largest[turn][w]);
+                turn ^= 1;
+            }
+            const float need = cache_scale_for(__uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(a))));
             const bool kept = o > 0 && was > 0.f && was < INFINITY;
             now = kept ? fmaxf(was, need) : need;
             grown = kept && now != was;
-            if (lane == 0 && !(kept && now == was)) *const_cast<float *>(scale) = now;
+            if (lane == 0 && sub == 0 && !(kept && now == was)) *const_cast<float *>(scale) = now;
         };
         typedef CacheRaw<T, E> Row;
         constexpr int RPI = 64 / LPR;             // rows at a time
@@ -328,12 +347,12 @@ __global__ __launch_bounds__(kCacheThreads, 4) void cache_append_kernel(AppendPa
             float a = 0.f;
             Row r[kAppendRows] = {};
             // (a run of a few rows, the usual one of a decoding step, is one vector)
-            const bool few = n <= RPI, fits = n <= kAppendRows * RPI;
+            const bool few = n <= RPI, fits = n <= of * kAppendRows * RPI;
             if (few) {
                 r[0] = row_at(first);
                 a = finite_max(r[0].get(), a);
             } else {
-                for (int i = first; i < n; i += kAppendRows * RPI) {
+                for (int i = first + sub * kAppendRows * RPI; i < n; i += of * kAppendRows * RPI) {
 #pragma unroll
                     for (int j = 0; j < kAppendRows; ++j) r[j] = row_at(i + j * RPI);
 #pragma unroll
@@ -349,10 +368,10 @@ __global__ __launch_bounds__(kCacheThreads, 4) void cache_append_kernel(AppendPa
                 if (j == 0 || !few) r[j].settle();
             with_quotient(now, [&](const auto &quotient) {
                 if (few) {
-                    store(r[0], first, quotient);
+                    if (sub == 0) store(r[0], first, quotient);
                     return;
                 }
-                for (int i = first; i < n; i += kAppendRows * RPI) {
+                for (int i = first + sub * kAppendRows * RPI; i < n; i += of * kAppendRows * RPI) {
                     if (!fits)
 #pragma unroll
                         for (int j = 0; j < kAppendRows; ++j) r[j] = row_at(i + j * RPI);
@@ -365,7 +384,7 @@ __global__ __launch_bounds__(kCacheThreads, 4) void cache_append_kernel(AppendPa
             });
             if (grown) {
                 const float shrink = was / now;
-                for (int i = lane / (D / 4); i < o; i += 64 / (D / 4)) {
+                for (int i = sub * (64 / (D / 4)) + lane / (D / 4); i < o; i += of * (64 / (D / 4))) {
                     uint32_t *c = (uint32_t *)(k + (int64_t)i * p.cache.k_st + lane % (D / 4) * 4);
                     *c = cache_rescale(*c, shrink);
                 }
@@ -393,7 +412,7 @@ __global__ __launch_bounds__(kCacheThreads, 4) void cache_append_kernel(AppendPa
 #pragma unroll
                 for (int i = 0; i < 16; ++i) a = finite_max(r[i].get(), a);
             } else {
-                for (int i = lane / LPR; i < n; i += 4 * RPI) {
+                for (int i = sub * 4 * RPI + lane / LPR; i < n; i += of * 4 * RPI) {
                     Row y[4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) y[j] = row_at(i + j * RPI);
@@ -407,7 +426,8 @@ __global__ __launch_bounds__(kCacheThreads, 4) void cache_append_kernel(AppendPa
             const float shrink = was / now;
             const bool again = !fits || grown;
             with_quotient(now, [&](const auto &quotient) {
-                for (int g = (grown ? 0 : g0) + (again ? lane / LPC : 0); g < g1; g += again ? 64 / LPC : 1) {
+                // (a group at hand is every wave's)
+                for (int g = (grown ? 0 : g0) + (again ? sub * (64 / LPC) + lane / LPC : sub); g < g1; g += again ? of * (64 / LPC) : of) {
                     if (again) {
                         c0 = v + (int64_t)d * p.cache.v_sd + g * 16, c1 = c0 + p.cache.v_sd;
                         a0 = *(Codes *)c0, a1 = *(Codes *)c1;

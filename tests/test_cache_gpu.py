@@ -447,7 +447,8 @@ def _slots_of(cache, page, b, first, count):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
-@pytest.mark.parametrize("dim,page,kv_heads", [(32, 16, 3), (64, 32, 2), (128, 16, 1), (128, 256, 2), (64, 128, 1)])
+@pytest.mark.parametrize("dim,page,kv_heads", [(32, 16, 3), (64, 32, 2), (128, 16, 1), (128, 256, 2), (64, 128, 1),
+                                               (32, 256, 2), (128, 64, 3)])
 def test_append(device, dtype, dim, page, kv_heads):
     """Runs of one token, of part of a page, over several pages, in the middle of a page whose scale has to grow or not;
     skipped slots between and around them; views of a packed projection."""
@@ -500,11 +501,11 @@ def test_append_forgets_a_page_that_starts_anew(device):
         _append_both(cache, x, x, _slots_of(cache, 16, 0, 20, 1), f"scale {bad}")
 
 
-def test_append_many_runs(device):
-    """More runs than a launch has waves for, in one call."""
+@pytest.mark.parametrize("page,batch", [(16, 700), (64, 300), (256, 4), (256, 3), (64, 1)])
+def test_append_many_runs(device, page, batch):
+    """More runs than a launch has waves for, in one call, and so few or many in large pages that waves share them or not."""
     import torch
 
-    page, batch = 16, 700
     cache = Cache([page] * batch, 9, page, 32, seed=23)
     slot = np.array([cache.table[b, 0] * page + b % page for b in range(batch)])
     x = torch.from_numpy(np.random.default_rng(24).normal(size=(batch, 2, 9, 32))).to(torch.float16).to("cuda:0")
