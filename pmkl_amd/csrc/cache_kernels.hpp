@@ -243,8 +243,8 @@ __device__ __forceinline__ uint32_t byte_mask(int at, int from, int to) {
 // requests nor their lengths.  Values are transposed on the way: a lane has two
 // columns and 16 tokens of a page, and stores each column's 16 codes as one
 // vector, with the codes around the run read first.  Bound by latency: a decoding
-// step of 256 requests, bf16, 8 heads of 128, 7.4 us (slots, then rows, scales and codes,
-// then stores); 4 prompts of 2,048 tokens, 51 MB, 16.8 us, 3.0 TB/s.
+// step of 256 requests, bf16, 8 heads of 128, 7.0 us (slots, then rows, scales and codes,
+// then stores); 4 prompts of 2,048 tokens, 51 MB, 15.4 us, 3.3 TB/s.
 // In pages of 64 tokens and more a wave would read and write for long: where no more
 // than three runs begin among the 64 tokens, a workgroup's waves take a (run, head,
 // keys or values) together, a share of its rows each, in pages of 64 only while the
